@@ -301,6 +301,62 @@ int cla_cooc(cla_handle h, int32_t groupA, int32_t groupB, int64_t* out);
  * preAgg[i, code(r)] += Y[i, r]. */
 int cla_preagg(cla_handle h, int32_t group, const double* Y, int32_t nRowY, double* preAgg);
 
+/* ---- products of layers: 8-bit matrices and gated units ----
+ * What a network over the same data adds to the products above. Weights W are nRows x nCols as in Y %*% X: a row of Y has nRows values,
+ * the output nCols. Operands and outputs are row-major with a leading dimension in elements, of one of the types below; device pointers are
+ * aligned to their elements (int8 operands and workspaces to 16 bytes). Work is queued on a stream, nothing is allocated and nothing waited
+ * for in the `_dev_async` forms, so that they can be captured into a graph; workspaces belong to the caller: calls that may run at the same
+ * time (other streams, other graphs) take workspaces of their own. Operands, outputs and workspaces do not overlap. nRowY may be 0. */
+enum cla_type { CLA_F64 = 0, CLA_F32 = 1, CLA_BF16 = 2, CLA_F16 = 3 };
+/* Activations: 1 / (1 + exp(-x)), x / (1 + exp(-x)), x Phi(x), its tanh approximation, max(x, 0), x. */
+enum cla_act { CLA_ACT_SIGMOID = 0, CLA_ACT_SILU = 1, CLA_ACT_GELU = 2, CLA_ACT_GELU_TANH = 3, CLA_ACT_RELU = 4, CLA_ACT_NONE = 5 };
+
+/* Rows to 8 bits: scale[i] = max |Y[i, :]| / 127 in fp32, q[i, k] = Y[i, k] / scale[i] rounded to the nearest whole number, ties to even, within
+ * -127 .. 127. A row of zeros has scale 0 and zeros; a row with a value that is not finite in fp32 the scale NaN and zeros (products with it are NaN).
+ * The rows of dQ are ldQ bytes apart, of which the first k are written. No counterpart in the reference. Returns 0 or a negative error. */
+int cla_quantize_rows_dev_async(const void* dY, int32_t type, int64_t nRowY, int32_t k, int64_t ldY, int8_t* dQ, int64_t ldQ, float* dScale,
+	void* hipStream);
+/* The same for all rows of a compressed block, decoded in chunks (at most 64 MiB of scratch kept with the block) on its stream: what a layer with
+ * many outputs takes instead of X %*% B. Returns 0 or a negative error without waiting for the stream. */
+int cla_block_quantize_rows_dev_async(cla_handle h, int8_t* dQ, int64_t ldQ, float* dScale);
+
+/* An 8-bit matrix resident in HBM: W[k, j] = values[k, j] * scales[j]. nRows <= 131,071 (sums of products stay exact in 32 bits).
+ * Calls on one handle are serialised, calls on different handles thread safe. */
+typedef struct cla_q8* cla_q8_handle;
+cla_q8_handle cla_q8_create(int64_t nRows, int32_t nCols);
+void cla_q8_free(cla_q8_handle h);
+int cla_q8_set_stream(cla_q8_handle h, void* hipStream);
+/* Sets the matrix from fp64 (host) or any type (device), each column quantised as cla_quantize_rows_dev_async does rows; or from values and scales
+ * as they are (any int8). byColumn != 0: the array has a row per column (nCols x nRows, ld >= nRows), else it is nRows x nCols (ld >= nCols).
+ * These wait for the handle's stream. */
+int cla_q8_set(cla_q8_handle h, const double* W);
+int cla_q8_set_dev(cla_q8_handle h, const void* dW, int32_t type, int64_t ld, int32_t byColumn);
+int cla_q8_set_values(cla_q8_handle h, const int8_t* values, const float* scales);
+int cla_q8_set_values_dev(cla_q8_handle h, const int8_t* dValues, int64_t ld, int32_t byColumn, const float* dScales);
+/* The values (nRows x nCols) and scales held. Waits for the stream. */
+int cla_q8_get(cla_q8_handle h, int8_t* values, float* scales);
+int64_t cla_q8_num_rows(cla_q8_handle h);
+int32_t cla_q8_num_cols(cla_q8_handle h);
+int64_t cla_q8_device_bytes(cla_q8_handle h);
+
+/* out[nRowY x nCols] = Y %*% W (+ bias per column), Y quantised row by row in the call; bias (may be null) and out have Y's type. The workspace
+ * holds at least cla_q8_workspace(h, nRowY) bytes. */
+int64_t cla_q8_workspace(cla_q8_handle h, int64_t nRowY);
+int cla_q8_lmm_dev_async(cla_q8_handle h, const void* dY, int32_t type, int64_t nRowY, int64_t ldY, const void* dBias, void* dOut, int64_t ldOut,
+	void* dWorkspace, int64_t workspaceBytes);
+/* The same with rows quantised before: dQ holds nRowY x ldQ bytes, ldQ a multiple of 16; bias and out have `type`. */
+int cla_q8_lmm_quantized_dev_async(cla_q8_handle h, const int8_t* dQ, int64_t ldQ, const float* dScale, int64_t nRowY, const void* dBias,
+	void* dOut, int32_t type, int64_t ldOut);
+/* The gated unit on a matrix of an even number of columns: out[nRowY x nCols / 2] = act(Y %*% Wg + bg) * (Y %*% Wu + bu), Wg the first half of the
+ * columns, Wu the second, bias both halves'. One kernel behind the quantisation. */
+int cla_q8_gate_dev_async(cla_q8_handle h, int32_t act, const void* dY, int32_t type, int64_t nRowY, int64_t ldY, const void* dBias, void* dOut,
+	int64_t ldOut, void* dWorkspace, int64_t workspaceBytes);
+int cla_q8_gate_quantized_dev_async(cla_q8_handle h, int32_t act, const int8_t* dQ, int64_t ldQ, const float* dScale, int64_t nRowY,
+	const void* dBias, void* dOut, int32_t type, int64_t ldOut);
+/* Host forms, fp64, dense: return the number of non-zeros of the output or a negative error. */
+int64_t cla_q8_lmm(cla_q8_handle h, const double* Y, int64_t nRowY, const double* bias, double* out);
+int64_t cla_q8_gate(cla_q8_handle h, int32_t act, const double* Y, int64_t nRowY, const double* bias, double* out);
+
 /* ---- introspection (the twin of the reference's -stats timers,
  * utils/DMLCompressionStatistics.java:44-125) ---- */
 /* enable != 0: bracket every kernel of this block with HIP events on its stream. */

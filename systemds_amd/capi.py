@@ -20,6 +20,9 @@ _f64p = C.POINTER(C.c_double)
 ERR_INVALID, ERR_UNSUPPORTED, ERR_DEVICE, ERR_STATE = -1, -2, -3, -4
 # product bits of cla_block_prepare
 PRODUCT_RMM, PRODUCT_LMM, PRODUCT_TSMM = 1, 2, 4
+# element types and activations of the layers' products (enum cla_type, enum cla_act)
+TYPES = {"f64": 0, "f32": 1, "bf16": 2, "f16": 3}
+ACTIVATIONS = {"sigmoid": 0, "silu": 1, "gelu": 2, "gelu_tanh": 3, "relu": 4, "none": 5}
 
 
 class ClaError(RuntimeError):
@@ -80,6 +83,28 @@ SIGNATURES = {
     "cla_counts": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p]),
     "cla_cooc": (C.c_int, [C.c_void_p, C.c_int32, C.c_int32, C.c_void_p]),
     "cla_preagg": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p]),
+    "cla_quantize_rows_dev_async": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "cla_block_quantize_rows_dev_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "cla_q8_create": (C.c_void_p, [C.c_int64, C.c_int32]),
+    "cla_q8_free": (None, [C.c_void_p]),
+    "cla_q8_set_stream": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "cla_q8_set": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "cla_q8_set_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32]),
+    "cla_q8_set_values": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "cla_q8_set_values_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p]),
+    "cla_q8_get": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
+    "cla_q8_num_rows": (C.c_int64, [C.c_void_p]),
+    "cla_q8_num_cols": (C.c_int32, [C.c_void_p]),
+    "cla_q8_device_bytes": (C.c_int64, [C.c_void_p]),
+    "cla_q8_workspace": (C.c_int64, [C.c_void_p, C.c_int64]),
+    "cla_q8_lmm_dev_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64]),
+    "cla_q8_lmm_quantized_dev_async": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64]),
+    "cla_q8_gate_dev_async": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64,
+                                        C.c_void_p, C.c_int64]),
+    "cla_q8_gate_quantized_dev_async": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int32,
+                                                  C.c_int64]),
+    "cla_q8_lmm": (C.c_int64, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "cla_q8_gate": (C.c_int64, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "cla_block_profile": (C.c_int, [C.c_void_p, C.c_int]),
     "cla_stats": (C.c_int, [C.c_void_p, C.c_char_p, C.c_size_t]),
     "cla_selftest_exception": (C.c_int, [C.c_int]),
@@ -377,6 +402,10 @@ class ClaBlock:
     def decompress_dev(self, dOut_ptr):
         return _check(self.lib.cla_decompress_dev(self.h, C.c_void_p(dOut_ptr)))
 
+    def quantize_rows_dev_async(self, dQ_ptr, ldQ, dScale_ptr):
+        """cla_block_quantize_rows_dev_async: all rows of the block in 8 bits, with their scales."""
+        return _check(self.lib.cla_block_quantize_rows_dev_async(self.h, dQ_ptr, ldQ, dScale_ptr))
+
     def profile(self, enable=True):
         _check(self.lib.cla_block_profile(self.h, 1 if enable else 0))
 
@@ -392,3 +421,93 @@ def build_block(n_rows, n_cols, specs):
     for s in specs:
         b.add(s)
     return b.finalize()
+
+
+# ---- products of layers: 8-bit matrices and gated units (pointers to device memory; types from TYPES, activations from ACTIVATIONS) ----
+def quantize_rows_dev_async(dY_ptr, type_, n_row_y, k, ldY, dQ_ptr, ldQ, dScale_ptr, stream=None):
+    """cla_quantize_rows_dev_async: rows to 8 bits, a scale each."""
+    return _check(load_library().cla_quantize_rows_dev_async(dY_ptr, type_, n_row_y, k, ldY, dQ_ptr, ldQ, dScale_ptr, stream))
+
+
+class ClaQ8:
+    """A device-resident 8-bit matrix with a scale per column (thin handle wrapper)."""
+
+    def __init__(self, n_rows, n_cols):
+        if not _initialised:
+            init(0)
+        self.lib = load_library()
+        self.n_rows, self.n_cols = int(n_rows), int(n_cols)
+        self.h = self.lib.cla_q8_create(self.n_rows, self.n_cols)
+        if not self.h:
+            raise ClaError(-1, last_error())
+
+    def close(self):
+        if self.h:
+            self.lib.cla_q8_free(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def set_stream(self, stream_ptr):
+        _check(self.lib.cla_q8_set_stream(self.h, stream_ptr))
+
+    def set(self, W):
+        """cla_q8_set: from fp64, n_rows x n_cols, quantised column by column."""
+        _check(self.lib.cla_q8_set(self.h, _ptr(_arr(W, np.float64).reshape(self.n_rows, self.n_cols))))
+        return self
+
+    def set_dev(self, dW_ptr, type_, ld, by_column=False):
+        _check(self.lib.cla_q8_set_dev(self.h, dW_ptr, type_, ld, int(by_column)))
+        return self
+
+    def set_values(self, values, scales):
+        """cla_q8_set_values: int8 values, n_rows x n_cols, and fp32 scales as they are."""
+        v, s = _arr(values, np.int8).reshape(self.n_rows, self.n_cols), _arr(scales, np.float32).reshape(self.n_cols)
+        _check(self.lib.cla_q8_set_values(self.h, _ptr(v), _ptr(s)))
+        return self
+
+    def set_values_dev(self, dValues_ptr, ld, dScales_ptr, by_column=False):
+        _check(self.lib.cla_q8_set_values_dev(self.h, dValues_ptr, ld, int(by_column), dScales_ptr))
+        return self
+
+    def get(self):
+        v, s = np.empty((self.n_rows, self.n_cols), np.int8), np.empty(self.n_cols, np.float32)
+        _check(self.lib.cla_q8_get(self.h, _ptr(v), _ptr(s)))
+        return v, s
+
+    def device_bytes(self):
+        return _check(self.lib.cla_q8_device_bytes(self.h))
+
+    def workspace(self, n_row_y):
+        """cla_q8_workspace: bytes that the products of so many rows need."""
+        return _check(self.lib.cla_q8_workspace(self.h, n_row_y))
+
+    def lmm_dev_async(self, dY_ptr, type_, n_row_y, ldY, dBias_ptr, dOut_ptr, ldOut, dWs_ptr, ws_bytes):
+        return _check(self.lib.cla_q8_lmm_dev_async(self.h, dY_ptr, type_, n_row_y, ldY, dBias_ptr, dOut_ptr, ldOut, dWs_ptr, ws_bytes))
+
+    def lmm_quantized_dev_async(self, dQ_ptr, ldQ, dScale_ptr, n_row_y, dBias_ptr, dOut_ptr, type_, ldOut):
+        return _check(self.lib.cla_q8_lmm_quantized_dev_async(self.h, dQ_ptr, ldQ, dScale_ptr, n_row_y, dBias_ptr, dOut_ptr, type_, ldOut))
+
+    def gate_dev_async(self, act, dY_ptr, type_, n_row_y, ldY, dBias_ptr, dOut_ptr, ldOut, dWs_ptr, ws_bytes):
+        return _check(self.lib.cla_q8_gate_dev_async(self.h, act, dY_ptr, type_, n_row_y, ldY, dBias_ptr, dOut_ptr, ldOut, dWs_ptr, ws_bytes))
+
+    def gate_quantized_dev_async(self, act, dQ_ptr, ldQ, dScale_ptr, n_row_y, dBias_ptr, dOut_ptr, type_, ldOut):
+        return _check(self.lib.cla_q8_gate_quantized_dev_async(self.h, act, dQ_ptr, ldQ, dScale_ptr, n_row_y, dBias_ptr, dOut_ptr, type_, ldOut))
+
+    def lmm(self, Y, bias=None):
+        """cla_q8_lmm: Y %*% W (+ bias) on host arrays; (out, number of non-zeros)."""
+        Y = _arr(Y, np.float64).reshape(-1, self.n_rows)
+        b = None if bias is None else _arr(bias, np.float64).reshape(self.n_cols)
+        out = np.empty((Y.shape[0], self.n_cols), np.float64)
+        return out, _check(self.lib.cla_q8_lmm(self.h, _ptr(Y), Y.shape[0], _ptr(b), _ptr(out)))
+
+    def gate(self, act, Y, bias=None):
+        """cla_q8_gate: act(Y %*% Wg) * (Y %*% Wu) on host arrays; (out, number of non-zeros)."""
+        Y = _arr(Y, np.float64).reshape(-1, self.n_rows)
+        b = None if bias is None else _arr(bias, np.float64).reshape(self.n_cols)
+        out = np.empty((Y.shape[0], self.n_cols // 2), np.float64)
+        return out, _check(self.lib.cla_q8_gate(self.h, ACTIVATIONS[act] if isinstance(act, str) else act, _ptr(Y), Y.shape[0], _ptr(b), _ptr(out)))

@@ -12,18 +12,6 @@
 #include <new>
 #include <stdexcept>
 
-// No exception may cross the C ABI (a JNI or FFM caller would abort the JVM instead of falling
-// back): every exported function runs its body between these two.
-#define CLA_TRY try {
-#define CLA_CATCH_BODY(onAlloc, onOther)                                                          \
-	}                                                                                             \
-	catch(const std::bad_alloc&) { cla::set_error("host memory allocation failed"); onAlloc; }   \
-	catch(const std::exception& e) { cla::set_error("unexpected exception: %s", e.what()); onOther; } \
-	catch(...) { cla::set_error("unexpected exception"); onOther; }
-#define CLA_CATCH_CODE(T) CLA_CATCH_BODY(return (T) -CLA_ERR_DEVICE, return (T) -CLA_ERR_INVALID)
-#define CLA_CATCH_NULL CLA_CATCH_BODY(return nullptr, return nullptr)
-#define CLA_CATCH_VOID CLA_CATCH_BODY(return, return)
-
 // Workspace of the entry point that allocates nothing (cla_rmm_dev_noalloc): the non-zero counter in the
 // first NNZ_BYTES, then the pre-aggregated tables. One copy per GPU, held until the process ends. In host
 // code the name is only a handle for hipGetSymbolAddress: kernels get the address looked up at cla_init.
@@ -174,7 +162,7 @@ static void free_group(HostGroup& g) {
 	g.owned.clear();
 }
 
-static int check_ready() {
+int check_ready() {
 	if(g_device < 0) {
 		set_error("cla_init has not been called (or failed): no HIP device selected");
 		return -CLA_ERR_STATE;

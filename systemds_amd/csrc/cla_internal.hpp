@@ -7,6 +7,8 @@
 #include <mutex>
 #include <atomic>
 #include <functional>
+#include <new>
+#include <stdexcept>
 #include <string>
 #include <vector>
 
@@ -260,9 +262,22 @@ struct cla_block {
 	bool poisoned = false;           // a failed finalize left the block half built: only free is allowed
 };
 
+// No exception may cross the C ABI (a JNI or FFM caller would abort the JVM instead of falling
+// back): every exported function runs its body between these two.
+#define CLA_TRY try {
+#define CLA_CATCH_BODY(onAlloc, onOther)                                                          \
+	}                                                                                             \
+	catch(const std::bad_alloc&) { cla::set_error("host memory allocation failed"); onAlloc; }   \
+	catch(const std::exception& e) { cla::set_error("unexpected exception: %s", e.what()); onOther; } \
+	catch(...) { cla::set_error("unexpected exception"); onOther; }
+#define CLA_CATCH_CODE(T) CLA_CATCH_BODY(return (T) -CLA_ERR_DEVICE, return (T) -CLA_ERR_INVALID)
+#define CLA_CATCH_NULL CLA_CATCH_BODY(return nullptr, return nullptr)
+#define CLA_CATCH_VOID CLA_CATCH_BODY(return, return)
+
 namespace cla {
 
 void set_error(const char* fmt, ...);
+int check_ready(); // cla_init has been called, and the device it chose is the current one
 extern int g_ldsPerBlock;   // usable LDS bytes per workgroup
 // Lets a kernel take up to the device's LDS per workgroup as dynamic shared memory; said once per kernel (a value
 // per call could be lowered by a caller on another handle between a call's setting and its launch).

@@ -1,0 +1,373 @@
+// Tiles of a product of two matrices held by rows of the summed index: D[i, j] = sum_k A[i, k] * B[j, k], for 8-bit integers, 16-bit floats,
+// fp32 and fp64 alike. "Rows" (i, tokens or table rows) are the output's rows, "columns" (j) its columns: weights, one row of them per column.
+//
+// All types share one shape of tile, counted in bytes: a step takes 128 bytes of the summed index of every row and column of the tile through
+// LDS (128 int8, 64 16-bit, 32 fp32, 16 fp64 values), a lane's matrix operand is 16 bytes of one row. Which values of the summed index meet in
+// an instruction does not matter as long as both operands agree, so the fp32 and fp64 instructions, which take one value a lane, run once per
+// value of the 16 bytes. Columns are the instruction's A operand, rows its B operand: a lane's results are several columns of one row.
+//
+// LDS rows are 128 bytes apart; 16-byte piece c of row r lies at place c ^ (r % 8), so that eight lanes that read one piece of eight rows use
+// all banks. The copies to LDS write a wave's 1 KB in lane order: the exchange is made in the addresses that the lanes read from.
+#pragma once
+#include "cla_device.hpp"
+
+namespace cla {
+
+typedef int mm_i32x4 __attribute__((ext_vector_type(4)));
+typedef int mm_i32x16 __attribute__((ext_vector_type(16)));
+typedef float mm_f32x4 __attribute__((ext_vector_type(4)));
+typedef float mm_f32x16 __attribute__((ext_vector_type(16)));
+typedef double mm_f64x2 __attribute__((ext_vector_type(2)));
+typedef double mm_f64x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 mm_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 mm_f16x8 __attribute__((ext_vector_type(8)));
+
+// What a type's values are computed in: fp32, and fp64 for fp64.
+template <class T> struct MmCalc { typedef float type; };
+template <> struct MmCalc<double> { typedef double type; };
+
+// An operand type on the matrix cores. FR: rows of a fragment (16 bytes of FR rows in 64 lanes: 64 / FR pieces of the summed index);
+// place(r): the fragment's column of a lane's result r, less what col(lane) adds.
+template <class E> struct MmOp;
+template <> struct MmOp<int8_t> {
+	static constexpr int FR = 32;
+	typedef int Sum;
+	typedef mm_i32x16 Acc;
+	typedef mm_i32x4 Acc16;
+	static __device__ __forceinline__ void mma(Acc& c, mm_i32x4 a, mm_i32x4 b) { c = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) { c = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+};
+template <> struct MmOp<__bf16> {
+	static constexpr int FR = 32;
+	typedef float Sum;
+	typedef mm_f32x16 Acc;
+	typedef mm_f32x4 Acc16;
+	static __device__ __forceinline__ void mma(Acc& c, mm_i32x4 a, mm_i32x4 b) {
+		c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(mm_bf16x8, a), __builtin_bit_cast(mm_bf16x8, b), c, 0, 0, 0);
+	}
+	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) {
+		c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, a), __builtin_bit_cast(mm_bf16x8, b), c, 0, 0, 0);
+	}
+};
+template <> struct MmOp<_Float16> {
+	static constexpr int FR = 32;
+	typedef float Sum;
+	typedef mm_f32x16 Acc;
+	typedef mm_f32x4 Acc16;
+	static __device__ __forceinline__ void mma(Acc& c, mm_i32x4 a, mm_i32x4 b) {
+		c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(mm_f16x8, a), __builtin_bit_cast(mm_f16x8, b), c, 0, 0, 0);
+	}
+	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) {
+		c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(mm_f16x8, a), __builtin_bit_cast(mm_f16x8, b), c, 0, 0, 0);
+	}
+};
+template <> struct MmOp<float> {
+	static constexpr int FR = 32;
+	typedef float Sum;
+	typedef mm_f32x16 Acc;
+	typedef mm_f32x4 Acc16;
+	static __device__ __forceinline__ void mma(Acc& c, mm_i32x4 a, mm_i32x4 b) {
+		const mm_f32x4 x = __builtin_bit_cast(mm_f32x4, a), y = __builtin_bit_cast(mm_f32x4, b);
+#pragma unroll
+		for(int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
+	}
+	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) {
+		const mm_f32x4 x = __builtin_bit_cast(mm_f32x4, a), y = __builtin_bit_cast(mm_f32x4, b);
+#pragma unroll
+		for(int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+	}
+};
+template <> struct MmOp<double> {
+	static constexpr int FR = 16;
+	typedef double Sum;
+	typedef mm_f64x4 Acc;
+	typedef mm_f64x4 Acc16;
+	static __device__ __forceinline__ void mma(Acc& c, mm_i32x4 a, mm_i32x4 b) {
+		const mm_f64x2 x = __builtin_bit_cast(mm_f64x2, a), y = __builtin_bit_cast(mm_f64x2, b);
+#pragma unroll
+		for(int i = 0; i < 2; i++) c = __builtin_amdgcn_mfma_f64_16x16x4f64(x[i], y[i], c, 0, 0, 0);
+	}
+	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) { mma(c, a, b); }
+};
+
+// The column (of a fragment) that result r of this lane belongs to; its row is lane % FR. Results come in groups of neighbouring columns
+// (four, or one of fp64).
+template <class E>
+__device__ __forceinline__ int mm_col(int lane, int r) {
+	if(MmOp<E>::FR == 32) return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+	return 4 * r + (lane >> 4);
+}
+template <class E>
+__device__ __forceinline__ int mm_col16(int lane, int r) {
+	return std::is_same<E, double>::value ? 4 * r + (lane >> 4) : 4 * (lane >> 4) + r;
+}
+
+template <class T>
+__device__ __forceinline__ typename MmCalc<T>::type mm_in(T x) { return (typename MmCalc<T>::type) x; }
+
+// The activation of a gated unit and its derivative (act: enum cla_act). The logistic function of large negative arguments: exp overflows to
+// infinity and 1 / infinity is 0, the limit.
+__device__ __forceinline__ float mm_exp(float x) { return expf(x); }
+__device__ __forceinline__ double mm_exp(double x) { return exp(x); }
+__device__ __forceinline__ float mm_erf(float x) { return erff(x); }
+__device__ __forceinline__ double mm_erf(double x) { return erf(x); }
+__device__ __forceinline__ float mm_tanh(float x) { return tanhf(x); }
+__device__ __forceinline__ double mm_tanh(double x) { return tanh(x); }
+enum : int { ACT_SIGMOID = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_RELU = 4, ACT_NONE = 5 };
+template <class C>
+__device__ __forceinline__ C mm_act(C x, int act) {
+	switch(act) { // (uniform)
+		case ACT_SIGMOID: return C(1) / (C(1) + mm_exp(-x));
+		case ACT_SILU: return x / (C(1) + mm_exp(-x));
+		case ACT_GELU: return C(0.5) * x * (C(1) + mm_erf(x * C(0.70710678118654752440)));
+		case ACT_GELU_TANH: return C(0.5) * x * (C(1) + mm_tanh(C(0.79788456080286535588) * (x + C(0.044715) * x * x * x)));
+		case ACT_RELU: return x < C(0) ? C(0) : x; // (a NaN stays one)
+		default: return x;
+	}
+}
+template <class C>
+__device__ __forceinline__ C mm_act_slope(C x, int act) {
+	switch(act) {
+		case ACT_SIGMOID: { const C s = C(1) / (C(1) + mm_exp(-x)); return s * (C(1) - s); }
+		case ACT_SILU: { const C s = C(1) / (C(1) + mm_exp(-x)); return s * (C(1) + x * (C(1) - s)); }
+		case ACT_GELU: return C(0.5) * (C(1) + mm_erf(x * C(0.70710678118654752440))) + x * mm_exp(C(-0.5) * x * x) * C(0.39894228040143267794);
+		case ACT_GELU_TANH: {
+			const C c = C(0.79788456080286535588), t = mm_tanh(c * (x + C(0.044715) * x * x * x));
+			return C(0.5) * (C(1) + t) + C(0.5) * x * (C(1) - t * t) * c * (C(1) + C(0.134145) * x * x);
+		}
+		case ACT_RELU: return x > C(0) ? C(1) : C(0);
+		default: return C(1);
+	}
+}
+
+// 16 bytes of elements of ES bytes from any address of their alignment, `left` bytes of the row from there on: what lies behind the row is 0.
+template <int ES>
+__device__ __forceinline__ mm_i32x4 mm_load16(const char* p, int64_t left) {
+	mm_i32x4 v = {0, 0, 0, 0};
+	if(left >= 16) __builtin_memcpy(&v, p, 16);
+	else if(left > 0) {
+		if(ES == 8) { // (one of two)
+			uint64_t x;
+			__builtin_memcpy(&x, p, 8);
+			v[0] = (int) (uint32_t) x; v[1] = (int) (x >> 32);
+		}
+		else if(ES == 4) {
+#pragma unroll
+			for(int i = 0; i < 3; i++)
+				if(4 * i < left) { uint32_t x; __builtin_memcpy(&x, p + 4 * i, 4); v[i] = (int) x; }
+		}
+		else if(ES == 2) {
+#pragma unroll
+			for(int i = 0; i < 7; i++)
+				if(2 * i < left) { uint16_t x; __builtin_memcpy(&x, p + 2 * i, 2); v[i >> 1] |= (int) ((uint32_t) x << (16 * (i & 1))); }
+		}
+		else {
+#pragma unroll
+			for(int i = 0; i < 15; i++)
+				if(i < left) v[i >> 2] |= (int) ((uint32_t) (uint8_t) p[i] << (8 * (i & 3)));
+		}
+	}
+	return v;
+}
+
+struct MmArgs {
+	const char* rows;         // M rows, ldRows bytes apart
+	const char* cols;         // N columns (gated: the gate's N, then the other projection's N), ldCols bytes apart
+	int64_t ldRows, ldCols;
+	int64_t zRows, zCols;     // bytes between the operands of successive parts of the summed index (split)
+	int64_t M;
+	int32_t N;                // columns of the output
+	int64_t K, kPart;         // bytes of the summed index in all and of a part
+	int32_t tilesM, tilesN, parts;
+};
+
+constexpr unsigned MM_OUT = 0x70000000u; // an offset behind every operand's end: such a load is answered with zeros
+constexpr int64_t MM_MAX_LD = 4 << 20;   // bytes: a tile's offsets (256 rows) stay within 2^30
+
+// E: operands, TM x TN: rows and columns (gated: TN / 2 columns of either projection) of a tile, WM x WN waves. DIRECT: operands whose rows begin
+// and end at multiples of 16 bytes go from global memory to LDS without registers; others are loaded a step ahead into registers.
+template <class E, int TM, int TN, int WM, int WN, bool GATED, bool DIRECT, class Epi>
+__global__ __launch_bounds__(64 * WM * WN, TM * TN / (WM * WN) >= 128 * 128 ? 1 : 2) void k_mm(MmArgs A, Epi epi) {
+#ifdef __HIP_DEVICE_COMPILE__ // (the host pass knows no buffer descriptors)
+	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
+	typedef MmOp<E> Op;
+	constexpr int FR = Op::FR, NW = WM * WN, PIECES = 64 / FR, SUB = 8 / PIECES;
+	constexpr int SM = TM / WM, SN = TN / WN, MF = SM / FR, NF = SN / FR;
+	constexpr int LM = TM / 8 / NW, LN = TN / 8 / NW, BUF = (TM + TN) * 128;
+	static_assert(SUB % 2 == 0 && LM * 8 * NW == TM && LN * 8 * NW == TN && (!GATED || NF % 2 == 0), "tile");
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+
+	// Tiles go to the XCDs in runs (their L2s see neighbours), within a run 8 row tiles share each of the column tiles.
+	int tm, tn, part;
+	{
+		const unsigned n = gridDim.x, xcd = blockIdx.x % 8, at = blockIdx.x / 8, q = n / 8, rest = n % 8;
+		unsigned t = xcd * q + min(xcd, rest) + at;
+		const unsigned per = (unsigned) A.tilesM * (unsigned) A.tilesN;
+		part = (int) (t / per);
+		t -= (unsigned) part * per;
+		const unsigned width = 8u * (unsigned) A.tilesN, group = t / width, in = t - group * width, gm = min((unsigned) A.tilesM - group * 8u, 8u);
+		tm = (int) (group * 8u + in % gm);
+		tn = (int) (in / gm);
+	}
+	const int64_t m0 = (int64_t) tm * TM;
+	const int n0 = tn * (GATED ? TN / 2 : TN);
+	const int64_t left = A.K - (int64_t) part * A.kPart, K = left < A.kPart ? left : A.kPart; // bytes of this part
+	const int nk = (int) ((K + 127) >> 7);
+	const int rowsIn = (int) min(A.M - m0, (int64_t) TM), colsIn = min(A.N - n0, GATED ? TN / 2 : TN);
+	const char* const pRows = A.rows + part * A.zRows + m0 * A.ldRows;
+	const char* const pCols = A.cols + part * A.zCols + (int64_t) n0 * A.ldCols;
+	const char* const pUp = GATED ? pCols + (int64_t) A.N * A.ldCols : pCols;
+	const int ldR = (int) A.ldRows, ldC = (int) A.ldCols;
+
+	// a wave takes every NW-th 8 rows of the tile; lane: row lane / 8 of them, piece (lane % 8) ^ (lane / 8) of the step
+	const int lr = lane >> 3, piece = ((lane & 7) ^ lr) * 16;
+	auto col_half = [&](int i) { return GATED ? ((i * 8) / FR) & 1 : 0; };                     // gate's or the other projection's
+	auto col_row = [&](int i) { return GATED ? ((i * 8) / (2 * FR)) * FR + (i * 8) % FR : i * 8; }; // first of 8 columns
+	__amdgpu_buffer_rsrc_t rRows, rCols, rUp;
+	if(DIRECT) {
+		rRows = __builtin_amdgcn_make_buffer_rsrc((void*) pRows, 0, rowsIn * ldR, 0x00020000);
+		rCols = __builtin_amdgcn_make_buffer_rsrc((void*) pCols, 0, colsIn * ldC, 0x00020000);
+		if(GATED) rUp = __builtin_amdgcn_make_buffer_rsrc((void*) pUp, 0, colsIn * ldC, 0x00020000);
+	}
+	mm_i32x4 hold[DIRECT ? 1 : LM + LN];
+	auto issue = [&](int t) { // step t's operands: on their way to LDS (buffer t % 2), or into registers
+		const int k = t * 128;
+		if(DIRECT) {
+			char* const to = mm_smem + (t & 1) * BUF;
+			const bool out = k + piece >= K;
+			const unsigned vr = out ? MM_OUT : (unsigned) (lr * ldR + piece), vc = out ? MM_OUT : (unsigned) (lr * ldC + piece);
+#pragma unroll
+			for(int j = 0; j < LM; j++) {
+				const int i = j * NW + wave;
+				__builtin_amdgcn_raw_ptr_buffer_load_lds(rRows, (__attribute__((address_space(3))) void*) (to + i * 1024), 16, (int) (vr + (unsigned) (i * 8 * ldR)), k, 0, 0);
+			}
+#pragma unroll
+			for(int j = 0; j < LN; j++) {
+				const int i = j * NW + wave;
+				__builtin_amdgcn_raw_ptr_buffer_load_lds(col_half(i) ? rUp : rCols, (__attribute__((address_space(3))) void*) (to + TM * 128 + i * 1024), 16,
+					(int) (vc + (unsigned) (col_row(i) * ldC)), k, 0, 0);
+			}
+		}
+		else {
+#pragma unroll
+			for(int j = 0; j < LM; j++) {
+				const int r = (j * NW + wave) * 8 + lr;
+				hold[j] = mm_load16<sizeof(E)>(pRows + (int64_t) r * ldR + k + piece, r < rowsIn ? K - k - piece : 0);
+			}
+#pragma unroll
+			for(int j = 0; j < LN; j++) {
+				const int i = j * NW + wave, c = col_row(i) + lr;
+				hold[LM + j] = mm_load16<sizeof(E)>((col_half(i) ? pUp : pCols) + (int64_t) c * ldC + k + piece, c < colsIn ? K - k - piece : 0);
+			}
+		}
+	};
+	auto put = [&](int t) { // the registers' step into LDS
+		char* const to = mm_smem + (t & 1) * BUF + lane * 16;
+#pragma unroll
+		for(int j = 0; j < LM; j++) *(mm_i32x4*) (to + (j * NW + wave) * 1024) = hold[j];
+#pragma unroll
+		for(int j = 0; j < LN; j++) *(mm_i32x4*) (to + TM * 128 + (j * NW + wave) * 1024) = hold[LM + j];
+	};
+
+	const int wm = wave % WM, wn = wave / WM;
+	typename Op::Acc acc[NF][MF];
+#pragma unroll
+	for(int i = 0; i < NF; i++)
+#pragma unroll
+		for(int j = 0; j < MF; j++)
+#pragma unroll
+			for(int r = 0; r < FR * FR / 64; r++) acc[i][j][r] = 0;
+	mm_i32x4 fc[2][NF], fr[2][MF];
+	const int fl = (lane % FR) * 128;
+	auto read = [&](int set, int t, int s) {
+		const char* const from = mm_smem + (t & 1) * BUF + fl + (((s * PIECES + lane / FR) ^ (lane & 7)) << 4);
+#pragma unroll
+		for(int j = 0; j < MF; j++) fr[set][j] = *(const mm_i32x4*) (from + (wm * SM + j * FR) * 128);
+#pragma unroll
+		for(int i = 0; i < NF; i++) fc[set][i] = *(const mm_i32x4*) (from + (TM + wn * SN + i * FR) * 128);
+	};
+	auto barrier = [&]() {
+		asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+		__builtin_amdgcn_s_barrier();
+		asm volatile("" ::: "memory");
+	};
+
+	if(nk > 0) {
+		issue(0);
+		if(DIRECT) {
+			if(nk > 1) {
+				issue(1);
+				asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LM + LN) : "memory");
+			}
+			else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+		}
+		else put(0);
+		barrier();
+		read(0, 0, 0);
+	}
+	for(int t = 0; t < nk; t++) {
+		if(!DIRECT && t + 1 < nk) issue(t + 1);
+#pragma unroll
+		for(int s = 0; s < SUB; s++) {
+			if(s + 1 < SUB) read((s + 1) & 1, t, s + 1);
+			else if(t + 1 < nk) {
+				// everything of step t has been read; step t + 1 was requested a step ago
+				if(DIRECT) {
+					asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+					barrier();
+					if(t + 2 < nk) issue(t + 2);
+				}
+				else {
+					put(t + 1); // (its buffer was last read in step t - 1)
+					barrier();
+				}
+				read(0, t + 1, 0);
+			}
+#pragma unroll
+			for(int i = 0; i < NF; i++)
+#pragma unroll
+				for(int j = 0; j < MF; j++) Op::mma(acc[i][j], fc[s & 1][i], fr[s & 1][j]);
+		}
+	}
+	barrier(); // LDS is the epilogue's
+	epi.template run<E, MF, NF, GATED>(acc, mm_smem + wave * Epi::template region<E, NF, GATED>(), m0 + wm * SM, n0 + wn * (GATED ? SN / 2 : SN), A.M, A.N, part, tm * WM + wm, lane);
+#endif
+}
+
+// The same for few rows (up to 16 MR): columns are a stream of bytes that is read once, from global memory straight into the matrix operand. A block
+// takes 16 columns (gated: of either projection), its waves take turns of the summed index and add their sums up in LDS, in the order of the waves.
+// Lane: column (and row) lane % 16, 16 bytes from 16 (lane / 16) on of every 64. Rows that are not there are zeros.
+constexpr int MMF_WAVES = 8, MMF_UNROLL = 4;
+template <class E, bool GATED, int MR, class Rows>
+__device__ __forceinline__ void mm_few(const char* cols, int64_t ldCols, int n0, int N, int64_t K, const Rows& rowOf, typename MmOp<E>::Acc16 (&acc)[GATED ? 2 : 1][MR],
+	int wave, int lane) {
+	typedef MmOp<E> Op;
+	constexpr int H = GATED ? 2 : 1;
+	const int l16 = lane & 15;
+	const int64_t at = (lane >> 4) * 16;
+	const int c = min(n0 + l16, N - 1);
+	const char* const p[2] = {cols + (int64_t) c * ldCols, cols + ((int64_t) c + (GATED ? N : 0)) * ldCols};
+#pragma unroll
+	for(int h = 0; h < H; h++)
+#pragma unroll
+		for(int j = 0; j < MR; j++) acc[h][j] = typename Op::Acc16{0, 0, 0, 0};
+	for(int64_t k = (int64_t) wave * 64 * MMF_UNROLL; k < K; k += MMF_WAVES * 64 * MMF_UNROLL) {
+		mm_i32x4 w[H][MMF_UNROLL], y[MR][MMF_UNROLL];
+#pragma unroll
+		for(int u = 0; u < MMF_UNROLL; u++)
+#pragma unroll
+			for(int h = 0; h < H; h++) w[h][u] = mm_load16<sizeof(E)>(p[h] + k + u * 64 + at, K - (k + u * 64 + at));
+#pragma unroll
+		for(int u = 0; u < MMF_UNROLL; u++)
+#pragma unroll
+			for(int j = 0; j < MR; j++) y[j][u] = rowOf(16 * j + l16, k + u * 64 + at, K - (k + u * 64 + at));
+#pragma unroll
+		for(int u = 0; u < MMF_UNROLL; u++)
+#pragma unroll
+			for(int h = 0; h < H; h++)
+#pragma unroll
+				for(int j = 0; j < MR; j++) Op::mma16(acc[h][j], w[h][u], y[j][u]);
+	}
+}
+
+} // namespace cla

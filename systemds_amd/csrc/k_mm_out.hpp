@@ -1,0 +1,103 @@
+// What a tile of k_mm.hpp does with its sums: a wave passes them through a region of LDS of its own, fragment of rows by fragment, so that everything
+// that follows (scales, biases, activations, stores) is done on neighbouring columns of a row, 16 bytes of the output at a time.
+#pragma once
+#include "k_mm.hpp"
+
+namespace cla {
+
+// n consecutive values as one access
+template <class T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) MmPack { T x[N]; };
+
+__device__ __forceinline__ void mm_wave_sync() { // what the wave's lanes wrote to LDS is there for its other lanes
+	__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+	__builtin_amdgcn_wave_barrier();
+}
+
+// The region: [half][row of the fragment][column], the halves of a gated unit apart.
+template <class E, int NF, bool GATED> struct MmRegion {
+	typedef typename MmOp<E>::Sum Sum;
+	static constexpr int FR = MmOp<E>::FR, H = GATED ? 2 : 1, COLS = NF * FR / H, R = FR * FR / 64, W = FR == 32 ? 4 : 1;
+	static constexpr int PITCH = COLS * (int) sizeof(Sum) + 16, HALF = FR * PITCH, BYTES = H * HALF;
+	template <int MF, class Acc>
+	static __device__ __forceinline__ void put(char* region, Acc (&acc)[NF][MF], int j, int lane) {
+#pragma unroll
+		for(int i = 0; i < NF; i++)
+#pragma unroll
+			for(int r = 0; r < R; r += W) {
+				MmPack<Sum, W> p;
+#pragma unroll
+				for(int v = 0; v < W; v++) p.x[v] = acc[i][j][r + v];
+				*(MmPack<Sum, W>*) (region + (i % H) * HALF + (lane % FR) * PITCH + ((i / H) * FR + mm_col<E>(lane, r)) * (int) sizeof(Sum)) = p;
+			}
+		mm_wave_sync();
+	}
+	static __device__ __forceinline__ Sum* at(char* region, int half, int row, int col) {
+		return (Sum*) (region + half * HALF + row * PITCH + col * (int) sizeof(Sum));
+	}
+};
+
+// V values to a row of the output, `cols` of them there
+template <class T, int V>
+__device__ __forceinline__ void mm_store(T* to, const T (&x)[V], int cols, bool aligned) {
+	if(aligned && cols >= V) {
+		MmPack<T, V> p;
+#pragma unroll
+		for(int v = 0; v < V; v++) p.x[v] = x[v];
+		*(MmPack<T, V>*) to = p;
+	}
+	else {
+#pragma unroll
+		for(int v = 0; v < V; v++)
+			if(v < cols) to[v] = x[v];
+	}
+}
+
+// The sums, times a scale for each row and column (SCALED: sums of 8-bit products), plus a bias for each column; gated: activation of the
+// gate's times the other projection's. Rounded to T once.
+template <class T, bool SCALED> struct MmEpiOut {
+	const float* sRow;
+	const float* sCol;
+	const T* bias;      // null: none
+	T* out;
+	int64_t ld;         // values
+	int32_t act;
+	int32_t aligned;    // out and its rows begin at multiples of 16 bytes
+
+	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
+	template <class E, int MF, int NF, bool GATED, class Acc>
+	__device__ __forceinline__ void run(Acc& acc, char* region, int64_t m0, int n0, int64_t M, int N, int, int, int lane) const {
+		typedef MmRegion<E, NF, GATED> Reg;
+		typedef typename MmCalc<T>::type C;
+		constexpr int FR = Reg::FR, H = Reg::H, V = 16 / (int) sizeof(T), PER = Reg::COLS / V;
+		static_assert(Reg::COLS % V == 0, "a row of the region is whole stores");
+		const int cols = N - n0;
+#pragma unroll
+		for(int j = 0; j < MF; j++) {
+			Reg::template put<MF>(region, acc, j, lane);
+			const int64_t row0 = m0 + j * FR;
+#pragma unroll 1
+			for(int i = lane; i < FR * PER; i += 64) {
+				const int r = i / PER, c = (i % PER) * V;
+				if(row0 + r >= M || c >= cols) continue;
+				const float sr = SCALED ? sRow[row0 + r] : 1.0f;
+				T x[V];
+#pragma unroll
+				for(int v = 0; v < V; v++) {
+					const int col = min(n0 + c + v, N - 1);
+					C y[H];
+#pragma unroll
+					for(int h = 0; h < H; h++) {
+						y[h] = (C) Reg::at(region, h, r, c)[v];
+						if(SCALED) y[h] *= (C) sr * (C) sCol[col + h * N];
+						if(bias) y[h] += (C) bias[col + h * N];
+					}
+					x[v] = (T) (GATED ? mm_act<C>(y[0], act) * y[H - 1] : y[0]);
+				}
+				mm_store<T, V>(out + (row0 + r) * ld + n0 + c, x, cols - c, aligned);
+			}
+			mm_wave_sync();
+		}
+	}
+};
+
+} // namespace cla
