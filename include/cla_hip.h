@@ -311,7 +311,7 @@ enum cla_type { CLA_F64 = 0, CLA_F32 = 1, CLA_BF16 = 2, CLA_F16 = 3 };
 /* Activations: 1 / (1 + exp(-x)), x / (1 + exp(-x)), x Phi(x), its tanh approximation, max(x, 0), x. */
 enum cla_act { CLA_ACT_SIGMOID = 0, CLA_ACT_SILU = 1, CLA_ACT_GELU = 2, CLA_ACT_GELU_TANH = 3, CLA_ACT_RELU = 4, CLA_ACT_NONE = 5 };
 
-/* Rows to 8 bits: scale[i] = max |Y[i, :]| / 127 in fp32, q[i, k] = Y[i, k] / scale[i] rounded to the nearest whole number, ties to even, within
+/* Rows to 8 bits: scale[i] = max |Y[i, :]| * (1 / 127), each in fp32, q[i, k] = Y[i, k] / scale[i] rounded to the nearest whole number, ties to even, within
  * -127 .. 127. A row of zeros has scale 0 and zeros; a row with a value that is not finite in fp32 the scale NaN and zeros (products with it are NaN).
  * The rows of dQ are ldQ bytes apart, of which the first k are written. No counterpart in the reference. Returns 0 or a negative error. */
 int cla_quantize_rows_dev_async(const void* dY, int32_t type, int64_t nRowY, int32_t k, int64_t ldY, int8_t* dQ, int64_t ldQ, float* dScale,
@@ -356,6 +356,23 @@ int cla_q8_gate_quantized_dev_async(cla_q8_handle h, int32_t act, const int8_t* 
 /* Host forms, fp64, dense: return the number of non-zeros of the output or a negative error. */
 int64_t cla_q8_lmm(cla_q8_handle h, const double* Y, int64_t nRowY, const double* bias, double* out);
 int64_t cla_q8_gate(cla_q8_handle h, int32_t act, const double* Y, int64_t nRowY, const double* bias, double* out);
+
+/* The gated unit in the operands' own type: out[nRowY x nOut] = act(Y %*% t(Wg) + bg) * (Y %*% t(Wu) + bu), W = rbind(Wg, Wu): 2 nOut x nIn, a row of
+ * weights per output column; bias (2 nOut) may be null. 16-bit and fp32 operands are summed in fp32, fp64 in fp64. One kernel. At most 4 MiB a row
+ * of Y and 1 MiB a row of the output. The workspace holds cla_gate_workspace(type, nRowY, nIn, nOut, 0) bytes (0: it may be null). */
+int64_t cla_gate_workspace(int32_t type, int64_t nRowY, int32_t nIn, int32_t nOut, int32_t backward);
+int cla_gate_dev_async(int32_t act, int32_t type, const void* dY, int64_t nRowY, int32_t nIn, int64_t ldY, const void* dW, int64_t ldW,
+	const void* dBias, int32_t nOut, void* dOut, int64_t ldOut, void* dWorkspace, int64_t workspaceBytes, void* hipStream);
+/* Its gradients from the incoming one (nRowY x nOut): of Y (nRowY x nIn), W (2 nOut x nIn) and bias (2 nOut); a null output is not computed. They
+ * are written, not added to, and do not depend on timing. The projections are computed again; the workspace holds
+ * cla_gate_workspace(type, nRowY, nIn, nOut, 1) bytes. */
+int cla_gate_backward_dev_async(int32_t act, int32_t type, const void* dY, int64_t nRowY, int32_t nIn, int64_t ldY, const void* dW, int64_t ldW,
+	const void* dBias, int32_t nOut, const void* dGrad, int64_t ldGrad, void* dGradY, int64_t ldGradY, void* dGradW, int64_t ldGradW,
+	void* dGradBias, void* dWorkspace, int64_t workspaceBytes, void* hipStream);
+/* Host forms, fp64, dense, on the null stream: the number of non-zeros of the output, 0 for the gradients, or a negative error. */
+int64_t cla_gate(int32_t act, const double* Y, int64_t nRowY, int32_t nIn, const double* W, const double* bias, int32_t nOut, double* out);
+int cla_gate_backward(int32_t act, const double* Y, int64_t nRowY, int32_t nIn, const double* W, const double* bias, int32_t nOut, const double* grad,
+	double* gradY, double* gradW, double* gradBias);
 
 /* ---- introspection (the twin of the reference's -stats timers,
  * utils/DMLCompressionStatistics.java:44-125) ---- */

@@ -105,6 +105,15 @@ SIGNATURES = {
                                                   C.c_int64]),
     "cla_q8_lmm": (C.c_int64, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     "cla_q8_gate": (C.c_int64, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
+    "cla_gate_workspace": (C.c_int64, [C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
+    "cla_gate_dev_async": (C.c_int, [C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32,
+                                     C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "cla_gate_backward_dev_async": (C.c_int, [C.c_int32, C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int32,
+                                              C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64,
+                                              C.c_void_p]),
+    "cla_gate": (C.c_int64, [C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
+    "cla_gate_backward": (C.c_int, [C.c_int32, C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_void_p]),
     "cla_block_profile": (C.c_int, [C.c_void_p, C.c_int]),
     "cla_stats": (C.c_int, [C.c_void_p, C.c_char_p, C.c_size_t]),
     "cla_selftest_exception": (C.c_int, [C.c_int]),
@@ -511,3 +520,46 @@ class ClaQ8:
         b = None if bias is None else _arr(bias, np.float64).reshape(self.n_cols)
         out = np.empty((Y.shape[0], self.n_cols // 2), np.float64)
         return out, _check(self.lib.cla_q8_gate(self.h, ACTIVATIONS[act] if isinstance(act, str) else act, _ptr(Y), Y.shape[0], _ptr(b), _ptr(out)))
+
+
+def gate_workspace(type_, n_row_y, n_in, n_out, backward):
+    """cla_gate_workspace: bytes of workspace of a gated unit's call."""
+    return _check(load_library().cla_gate_workspace(type_, n_row_y, n_in, n_out, int(backward)))
+
+
+def gate_dev_async(act, type_, dY_ptr, n_row_y, n_in, ldY, dW_ptr, ldW, dBias_ptr, n_out, dOut_ptr, ldOut, dWs_ptr=None, ws_bytes=0, stream=None):
+    """cla_gate_dev_async: act(Y t(Wg) + bg) * (Y t(Wu) + bu)."""
+    return _check(load_library().cla_gate_dev_async(act, type_, dY_ptr, n_row_y, n_in, ldY, dW_ptr, ldW, dBias_ptr, n_out, dOut_ptr, ldOut, dWs_ptr,
+                                                    ws_bytes, stream))
+
+
+def gate_backward_dev_async(act, type_, dY_ptr, n_row_y, n_in, ldY, dW_ptr, ldW, dBias_ptr, n_out, dGrad_ptr, ldGrad, dGradY_ptr, ldGradY, dGradW_ptr, ldGradW,
+                            dGradBias_ptr, dWs_ptr, ws_bytes, stream=None):
+    """cla_gate_backward_dev_async: the gradients of Y, W and bias (a null pointer leaves one out)."""
+    return _check(load_library().cla_gate_backward_dev_async(act, type_, dY_ptr, n_row_y, n_in, ldY, dW_ptr, ldW, dBias_ptr, n_out, dGrad_ptr, ldGrad, dGradY_ptr,
+                                                             ldGradY, dGradW_ptr, ldGradW, dGradBias_ptr, dWs_ptr, ws_bytes, stream))
+
+
+def gate(act, Y, W, bias=None):
+    """cla_gate on host arrays, W 2 n_out x n_in: (out, number of non-zeros)."""
+    if not _initialised:
+        init(0)
+    W = _arr(W, np.float64)
+    n_in, n_out = W.shape[1], W.shape[0] // 2
+    Y = _arr(Y, np.float64).reshape(-1, n_in)
+    b = None if bias is None else _arr(bias, np.float64).reshape(2 * n_out)
+    out = np.empty((Y.shape[0], n_out), np.float64)
+    return out, _check(load_library().cla_gate(ACTIVATIONS[act], _ptr(Y), Y.shape[0], n_in, _ptr(W), _ptr(b), n_out, _ptr(out)))
+
+
+def gate_backward(act, Y, W, grad, bias=None):
+    """cla_gate_backward on host arrays: (gradient of Y, of W, of bias)."""
+    if not _initialised:
+        init(0)
+    W = _arr(W, np.float64)
+    n_in, n_out = W.shape[1], W.shape[0] // 2
+    Y, grad = _arr(Y, np.float64).reshape(-1, n_in), _arr(grad, np.float64).reshape(-1, n_out)
+    b = None if bias is None else _arr(bias, np.float64).reshape(2 * n_out)
+    gy, gw, gb = np.empty_like(Y), np.empty_like(W), np.empty(2 * n_out)
+    _check(load_library().cla_gate_backward(ACTIVATIONS[act], _ptr(Y), Y.shape[0], n_in, _ptr(W), _ptr(b), n_out, _ptr(grad), _ptr(gy), _ptr(gw), _ptr(gb)))
+    return gy, gw, gb

@@ -1,6 +1,7 @@
 // Entry points of the 8-bit matrices (include/cla_hip.h): handles, checks of arguments, host forms. The kernels are in k_q8.hip.
 #include "../../include/cla_hip.h"
 #include "k_q8.hpp"
+#include "cla_layers.hpp"
 #include <algorithm>
 #include <cstring>
 
@@ -32,7 +33,6 @@ int check_act(const char* what, int act) {
 	return -CLA_ERR_INVALID;
 }
 
-// A row-major operand: there, aligned to `to` bytes, rows that do not overlap, their bytes within 63 bits.
 int check_operand(const char* what, const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld, size_t es, size_t to) {
 	if(!p || ((uintptr_t) p & (to - 1)) != 0) { set_error("%s: %s is %s", what, name, p ? "not aligned" : "null"); return -CLA_ERR_INVALID; }
 	if(ld < cols || ld > ((int64_t) 1 << 40) || rows > 0x7fffffffLL || ld * (double) es * (double) std::max<int64_t>(rows, 1) > 9e18) {
@@ -42,7 +42,7 @@ int check_operand(const char* what, const char* name, const void* p, int64_t row
 	return 0;
 }
 
-static int check_rows(const char* what, int64_t m) {
+int check_rows(const char* what, int64_t m) {
 	if(m >= 0 && m <= 0x7fffffffLL) return 0;
 	set_error("%s: %lld rows", what, (long long) m);
 	return -CLA_ERR_INVALID;
@@ -56,7 +56,6 @@ __global__ __launch_bounds__(256) void k_count_nonzero(const double* __restrict_
 	if((threadIdx.x & 63) == 0 && c != 0) atomicAdd(count, c);
 }
 
-// Non-zeros of n values on the device; waits for the stream.
 int64_t count_nonzero(const double* x, int64_t n, unsigned long long* dCount, hipStream_t stream) {
 	unsigned long long c = 0;
 	CLA_HIP(hipMemsetAsync(dCount, 0, sizeof(c), stream));
@@ -67,7 +66,6 @@ int64_t count_nonzero(const double* x, int64_t n, unsigned long long* dCount, hi
 	return (int64_t) c;
 }
 
-static size_t up(size_t x, size_t to) { return (x + to - 1) / to * to; }
 static int64_t ld_rows(const cla_q8* h) { return (int64_t) up((size_t) h->nRows, 16); }
 
 static int check_q8(cla_q8* h, bool set) {

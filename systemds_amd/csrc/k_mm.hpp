@@ -217,7 +217,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN / (WM * WN) >= 128 * 128 ? 1 
 	const char* const pRows = A.rows + part * A.zRows + m0 * A.ldRows;
 	const char* const pCols = A.cols + part * A.zCols + (int64_t) n0 * A.ldCols;
 	const char* const pUp = GATED ? pCols + (int64_t) A.N * A.ldCols : pCols;
-	const int ldR = (int) A.ldRows, ldC = (int) A.ldCols;
+	const int ldR = (int) A.ldRows, ldC = (int) A.ldCols; // (at most MM_MAX_LD, or 2^31 - 1 where offsets are not held in 32 bits)
 
 	// a wave takes every NW-th 8 rows of the tile; lane: row lane / 8 of them, piece (lane % 8) ^ (lane / 8) of the step
 	const int lr = lane >> 3, piece = ((lane & 7) ^ lr) * 16;

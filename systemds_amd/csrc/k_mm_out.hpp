@@ -62,10 +62,11 @@ template <class T, bool SCALED> struct MmEpiOut {
 	int64_t ld;         // values
 	int32_t act;
 	int32_t aligned;    // out and its rows begin at multiples of 16 bytes
+	int64_t zOut;       // values between the outputs of the parts of the summed index
 
 	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
 	template <class E, int MF, int NF, bool GATED, class Acc>
-	__device__ __forceinline__ void run(Acc& acc, char* region, int64_t m0, int n0, int64_t M, int N, int, int, int lane) const {
+	__device__ __forceinline__ void run(Acc& acc, char* region, int64_t m0, int n0, int64_t M, int N, int part, int, int lane) const {
 		typedef MmRegion<E, NF, GATED> Reg;
 		typedef typename MmCalc<T>::type C;
 		constexpr int FR = Reg::FR, H = Reg::H, V = 16 / (int) sizeof(T), PER = Reg::COLS / V;
@@ -93,9 +94,103 @@ template <class T, bool SCALED> struct MmEpiOut {
 					}
 					x[v] = (T) (GATED ? mm_act<C>(y[0], act) * y[H - 1] : y[0]);
 				}
-				mm_store<T, V>(out + (row0 + r) * ld + n0 + c, x, cols - c, aligned);
+				mm_store<T, V>(out + part * zOut + (row0 + r) * ld + n0 + c, x, cols - c, aligned);
 			}
 			mm_wave_sync();
+		}
+	}
+};
+
+// Backward pass of a gated unit: from the projections G, U (the sums) and the incoming gradient D to dG = D U act'(G) and dU = D act(G), rounded to T once.
+// They are written twice, by row (P: what dY sums over) and by column (Pt: what dW sums over, rows of the batch in parts of kPart), with zeros where
+// either is rounded up to whole 16 bytes; sums over the wave's rows, of the values before that rounding, for the biases' gradient.
+template <class T> struct MmEpiBack {
+	typedef typename MmCalc<T>::type C;
+	const T* bias;      // null: none
+	const T* D;
+	int64_t ldD;
+	T* P;               // null: not wanted
+	int64_t ldP;        // two halves of ldP / 2 columns, a multiple of 16 bytes each
+	T* Pt;              // null: not wanted
+	int64_t kPart;      // a multiple of 256
+	C* sums;            // null: not wanted; [wave's rows][2 N]
+	int32_t act;
+	int32_t alignedD;
+
+	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
+	template <class E, int MF, int NF, bool GATED, class Acc>
+	__device__ __forceinline__ void run(Acc& acc, char* region, int64_t m0, int n0, int64_t M, int N, int, int rowPart, int lane) const {
+		typedef MmRegion<E, NF, GATED> Reg;
+		constexpr int FR = Reg::FR, COLS = Reg::COLS, V = 16 / (int) sizeof(T), PER = COLS / V, S = (2 * COLS + 63) / 64;
+		static_assert(GATED && COLS % V == 0 && FR % V == 0, "two halves, whole stores both ways");
+		const int cols = N - n0, half = (int) (ldP / 2) - n0;
+		C sum[S];
+#pragma unroll
+		for(int s = 0; s < S; s++) sum[s] = C(0);
+#pragma unroll
+		for(int j = 0; j < MF; j++) {
+			Reg::template put<MF>(region, acc, j, lane);
+			const int64_t row0 = m0 + j * FR;
+#pragma unroll 1
+			for(int i = lane; i < FR * PER; i += 64) {
+				const int r = i / PER, c = (i % PER) * V;
+				const bool in = row0 + r < M && c < cols;
+				const T* const d = D + (row0 + r) * ldD + n0 + c;
+				T g[V], u[V];
+				MmPack<T, V> dv;
+				if(in && alignedD && c + V <= cols) dv = *(const MmPack<T, V>*) d;
+				else {
+#pragma unroll
+					for(int v = 0; v < V; v++) dv.x[v] = in && c + v < cols ? d[v] : (T) 0.0f;
+				}
+#pragma unroll
+				for(int v = 0; v < V; v++) {
+					C x = *Reg::at(region, 0, r, c + v), y = *Reg::at(region, 1, r, c + v);
+					if(bias) {
+						const int col = min(n0 + c + v, N - 1);
+						x += (C) bias[col]; y += (C) bias[col + N];
+					}
+					const bool there = in && c + v < cols;
+					const C dG = there ? (C) dv.x[v] * y * mm_act_slope<C>(x, act) : C(0), dU = there ? (C) dv.x[v] * mm_act<C>(x, act) : C(0);
+					*Reg::at(region, 0, r, c + v) = dG; *Reg::at(region, 1, r, c + v) = dU;
+					g[v] = (T) dG; u[v] = (T) dU;
+				}
+				if(P && row0 + r < M && c < half) {
+					T* const to = P + (row0 + r) * ldP + n0 + c;
+					mm_store<T, V>(to, g, V, true);
+					mm_store<T, V>(to + ldP / 2, u, V, true);
+				}
+			}
+			mm_wave_sync();
+			if(sums) {
+#pragma unroll
+				for(int s = 0; s < S; s++) {
+					const int i = s * 64 + lane;
+					if(i < 2 * COLS)
+						for(int r = 0; r < FR; r++) sum[s] += *Reg::at(region, i / COLS, r, i % COLS);
+				}
+			}
+			if(Pt && row0 < M) {
+				const int64_t part = row0 / kPart, at = row0 - part * kPart;
+				T* const to = Pt + part * 2 * N * kPart + at;
+#pragma unroll 1
+				for(int i = lane; i < 2 * COLS * (FR / V); i += 64) {
+					const int r = (i % (FR / V)) * V, c = i / (FR / V) % COLS, h = i / (FR / V) / COLS;
+					if(c >= cols || row0 + r >= M) continue;
+					MmPack<T, V> p;
+#pragma unroll
+					for(int v = 0; v < V; v++) p.x[v] = (T) *Reg::at(region, h, r + v, c);
+					*(MmPack<T, V>*) (to + (int64_t) (h * N + n0 + c) * kPart + r) = p;
+				}
+			}
+			mm_wave_sync();
+		}
+		if(sums && m0 < M) {
+#pragma unroll
+			for(int s = 0; s < S; s++) {
+				const int i = s * 64 + lane, c = i % COLS;
+				if(i < 2 * COLS && c < cols) sums[(int64_t) rowPart * 2 * N + (i / COLS) * N + n0 + c] = sum[s];
+			}
 		}
 	}
 };

@@ -1,5 +1,5 @@
 // 8-bit products with a scale for each row of Y and each column of W:
-//   out[i, j] = (sum_k q[i, k] * w[k, j]) * s[i] * t[j] (+ bias[j]),   q[i, k] = Y[i, k] / s[i] to the nearest whole number, s[i] = max |Y[i, :]| / 127
+//   out[i, j] = (sum_k q[i, k] * w[k, j]) * s[i] * t[j] (+ bias[j]),   q[i, k] = Y[i, k] / s[i] to the nearest whole number, s[i] = max |Y[i, :]| * (1 / 127)
 // and the gated unit act(out of the first half of the columns) * (out of the second half), one kernel. The sums of 8-bit products are exact in 32 bits
 // (at most 131,071 terms of 128 * 128), so an output carries the roundings of its scales' products and its own.
 #include "../../include/cla_hip.h"
@@ -42,11 +42,11 @@ __device__ __forceinline__ C q8_largest(const C (&x)[8], C m) {
 	return m;
 }
 
-// The scale of a row. A row with a value that is not finite, or whose largest is none in fp32, has the scale NaN (and zeros): its outputs are NaN.
+// The scale of a row: the largest times 1 / 127, both in fp32. A row with a value that is not finite, or whose largest is none in fp32, has the scale NaN (and zeros): its outputs are NaN.
 template <class C>
 __device__ __forceinline__ float q8_scale(C largest) {
 	const float a = (float) largest;
-	return a <= 3.4028234663852886e38f ? a / 127.0f : NAN;
+	return a <= 3.4028234663852886e38f ? a * (1.0f / 127.0f) : NAN;
 }
 
 // x / s to the nearest whole number, ties to even, as the exact quotient rounds. fp32: the product with the reciprocal is within one of it; x - r s is exact in
@@ -286,7 +286,7 @@ static int q8_mm(const Q8Product& p, hipStream_t stream) {
 	A.cols = (const char*) p.W; A.ldCols = p.ldW;
 	A.M = p.m; A.N = N; A.K = A.kPart = (p.K + 15) / 16 * 16; A.parts = 1;
 	const MmEpiOut<T, true> epi{p.s, p.t, (const T*) p.bias, (T*) p.out, p.ldOut, p.act,
-		(((uintptr_t) p.out | (uintptr_t) (p.ldOut * sizeof(T))) & 15) == 0};
+		(((uintptr_t) p.out | (uintptr_t) (p.ldOut * sizeof(T))) & 15) == 0, 0};
 	const int64_t n = GATED ? 2 * (int64_t) N : N, big = ((p.m + 255) / 256) * ((n + 255) / 256), mid = ((p.m + 127) / 128) * ((n + 127) / 128);
 	if(big >= g_numCU) return q8_tile<T, GATED, 256, 256>(A, epi, stream);
 	if(mid >= g_numCU) return q8_tile<T, GATED, 128, 128>(A, epi, stream);

@@ -31,11 +31,11 @@ def decode(b, t):
 
 
 def quantise(Y):
-    """(whole numbers, scales) of the rows of Y: max / 127 in fp32, exact quotients to the nearest, ties to even. fp64 quotients of fp32 operands and
+    """(whole numbers, scales) of the rows of Y: max * (1 / 127) in fp32, exact quotients to the nearest, ties to even. fp64 quotients of fp32 operands and
     of the fp64 values are what the definition says."""
     with np.errstate(all="ignore"):
         big = np.max(np.abs(Y), axis=1) if Y.shape[1] else np.zeros(Y.shape[0])
-        s = (big.astype(np.float32) / np.float32(127)).astype(np.float32)
+        s = big.astype(np.float32) * (np.float32(1) / np.float32(127))
         s[~np.isfinite(big.astype(np.float32))] = np.nan
         q = np.where(s[:, None] > 0, np.clip(np.rint(Y / s.astype(np.float64)[:, None]), -127, 127), 0.0)
     return np.nan_to_num(q).astype(np.int8), s

@@ -59,7 +59,7 @@ def test_quotients_next_to_a_half(cla, t):
     for i in range(257):
         e = rng.integers(lo, hi)
         top = decode(encode(np.array([(1 + rng.random()) * 2.0 ** e]), t), t)[0]
-        step = float(np.float32(top) / np.float32(127)) if top < 3e38 else top / 127
+        step = float(np.float32(top) * (np.float32(1) / np.float32(127))) if top < 3e38 else top / 127
         x = (rng.integers(-254, 255, 509) / 2.0) * step * (1 + rng.integers(-2, 3, 509) * 2.0 ** -24)
         x[0] = top
         Y[i] = np.clip(decode(encode(x, t), t), -top, top)

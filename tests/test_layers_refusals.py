@@ -37,3 +37,34 @@ def test_handles():
     assert b"null 8-bit matrix handle" in lib.cla_last_error()
     assert lib.cla_block_quantize_rows_dev_async(None, None, 8, None) == capi.ERR_INVALID
     lib.cla_q8_free(None)
+
+
+def test_gate():
+    from systemds_amd import capi
+    p = 1 << 20
+    names = ("act", "t", "y", "m", "k", "ldy", "w", "ldw", "b", "n")
+    good = (1, 1, p, 3, 8, 8, p, 8, None, 4)
+
+    def forward(out=p, ld=4, **kw):
+        return [kw.get(x, v) for x, v in zip(names, good)] + [out, ld]
+    for match, kw in [("activation 6", dict(act=6)), ("activation -1", dict(act=-1)), ("type 4", dict(t=4)), ("-1 rows", dict(m=-1)), ("weights of 0 x 4", dict(k=0)),
+                      ("weights of 8 x 0", dict(n=0)), ("Y is null", dict(y=None)), ("Y is not aligned", dict(y=p + 2)), ("leading dimension 7 of Y", dict(ldy=7)),
+                      ("W is null", dict(w=None)), ("leading dimension 7 of W", dict(ldw=7)), ("bias is not aligned", dict(b=p + 1)),
+                      ("the output is null", dict(out=None)), ("leading dimension 3 of the output", dict(ld=3))]:
+        refused(match, capi.gate_dev_async, *forward(**kw))
+
+    def backward(d=p, ldd=4, gy=p, ldgy=8, gw=p, ldgw=8, gb=p, **kw):
+        return [kw.get(x, v) for x, v in zip(names, good)] + [d, ldd, gy, ldgy, gw, ldgw, gb, p, 1 << 30]
+    for match, kw in [("activation 9", dict(act=9)), ("incoming gradient is null", dict(d=None)), ("dimension 3 of the incoming", dict(ldd=3)),
+                      ("dimension 7 of the gradient of Y", dict(ldgy=7)), ("dimension 7 of the gradient of W", dict(ldgw=7)), ("gradient of the bias", dict(gb=p + 1)),
+                      ("no gradient is asked for", dict(gy=None, gw=None, gb=None)), ("Y is null", dict(y=None))]:
+        refused(match, capi.gate_backward_dev_async, *backward(**kw))
+    for kw in (dict(k=(4 << 20) // 4 + 1, ldy=1 << 21, ldw=1 << 21), dict(n=(1 << 20) // 4 + 1)):
+        with pytest.raises(capi.ClaError, match="at most") as e:
+            capi.gate_dev_async(*forward(ld=1 << 21, **kw))
+        assert e.value.code == capi.ERR_UNSUPPORTED
+    with pytest.raises(capi.ClaError, match="2 GiB"):
+        capi.gate_dev_async(*forward(ldw=1 << 30))
+    refused("type 5", capi.gate_workspace, 5, 3, 8, 4, True)
+    refused("-3 rows", capi.gate_workspace, 1, -3, 8, 4, True)
+    assert capi.gate_workspace(1, 100, 8, 4, False) == 0 == capi.gate_workspace(1, 0, 8, 4, True) < capi.gate_workspace(1, 1, 8, 4, True)
