@@ -55,7 +55,7 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_gate_few(GateFew<T> A) {
 			for(int w = 0; w < MMF_WAVES; w++) x[h] += red[(w * 2 + h) * MR * 256 + i];
 			if(A.bias) x[h] += (C) A.bias[col + h * A.nOut];
 		}
-		A.out[row * A.ld + col] = (T) (mm_act<C>(x[0], A.act) * x[1]);
+		A.out[row * A.ld + col] = (T) (mm_act<T>(x[0], A.act) * x[1]);
 	}
 }
 

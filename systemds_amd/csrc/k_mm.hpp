@@ -6,8 +6,9 @@
 // an instruction does not matter as long as both operands agree, so the fp32 and fp64 instructions, which take one value a lane, run once per
 // value of the 16 bytes. Columns are the instruction's A operand, rows its B operand: a lane's results are several columns of one row.
 //
-// LDS rows are 128 bytes apart; 16-byte piece c of row r lies at place c ^ (r % 8), so that eight lanes that read one piece of eight rows use
-// all banks. The copies to LDS write a wave's 1 KB in lane order: the exchange is made in the addresses that the lanes read from.
+// LDS rows are 128 bytes apart, half of its 64 banks; 16-byte piece c of row r lies at place c ^ (r / 2 % 8), so that 16 lanes that read one piece of 16
+// rows use every bank once (with r % 8 in its place half of the LDS cycles were conflicts). The copies to LDS write a wave's 1 KB in lane order: the
+// exchange is made in the addresses that the lanes read from.
 #pragma once
 #include "cla_device.hpp"
 
@@ -102,41 +103,63 @@ __device__ __forceinline__ int mm_col16(int lane, int r) {
 	return std::is_same<E, double>::value ? 4 * r + (lane >> 4) : 4 * (lane >> 4) + r;
 }
 
-template <class T>
-__device__ __forceinline__ typename MmCalc<T>::type mm_in(T x) { return (typename MmCalc<T>::type) x; }
-
-// The activation of a gated unit and its derivative (act: enum cla_act). The logistic function of large negative arguments: exp overflows to
-// infinity and 1 / infinity is 0, the limit.
-__device__ __forceinline__ float mm_exp(float x) { return expf(x); }
-__device__ __forceinline__ double mm_exp(double x) { return exp(x); }
+// exp, 1 / x and tanh for values that are rounded to T: 16-bit results take the instructions for 2^x and 1 / x (a relative error below 2^-20 for arguments up to 16,
+// a thousandth of a bf16 rounding, a hundredth of an fp16 one), fp32 and fp64 the full functions.
+template <class T> struct MmMath {
+	typedef typename MmCalc<T>::type C;
+	static __device__ __forceinline__ C logistic(C x) { return C(1) / (C(1) + exp(-x)); } // (exp overflows to infinity, 1 / infinity is 0: the limit)
+	static __device__ __forceinline__ C gauss(C x) { return exp(C(-0.5) * x * x); }
+	static __device__ __forceinline__ C tanh_of(C x) { return tanh(x); }
+};
+template <> struct MmMath<float> {
+	static __device__ __forceinline__ float logistic(float x) { return 1.0f / (1.0f + expf(-x)); }
+	static __device__ __forceinline__ float gauss(float x) { return expf(-0.5f * x * x); }
+	static __device__ __forceinline__ float tanh_of(float x) { return tanhf(x); }
+};
+struct MmMathShort {
+	static __device__ __forceinline__ float logistic(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x)); }
+	static __device__ __forceinline__ float gauss(float x) { return __builtin_amdgcn_exp2f(-0.72134752044448170f * x * x); }
+	static __device__ __forceinline__ float tanh_of(float x) { return 2.0f * logistic(2.0f * x) - 1.0f; }
+};
+template <> struct MmMath<__bf16> : MmMathShort {};
+template <> struct MmMath<_Float16> : MmMathShort {};
 __device__ __forceinline__ float mm_erf(float x) { return erff(x); }
 __device__ __forceinline__ double mm_erf(double x) { return erf(x); }
-__device__ __forceinline__ float mm_tanh(float x) { return tanhf(x); }
-__device__ __forceinline__ double mm_tanh(double x) { return tanh(x); }
+
+// The activation of a gated unit (act: enum cla_act) and its derivative, for results of type T.
 enum : int { ACT_SIGMOID = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_RELU = 4, ACT_NONE = 5 };
-template <class C>
+template <class T, class C>
 __device__ __forceinline__ C mm_act(C x, int act) {
+	typedef MmMath<T> F;
 	switch(act) { // (uniform)
-		case ACT_SIGMOID: return C(1) / (C(1) + mm_exp(-x));
-		case ACT_SILU: return x / (C(1) + mm_exp(-x));
+		case ACT_SIGMOID: return F::logistic(x);
+		case ACT_SILU: return x * F::logistic(x);
 		case ACT_GELU: return C(0.5) * x * (C(1) + mm_erf(x * C(0.70710678118654752440)));
-		case ACT_GELU_TANH: return C(0.5) * x * (C(1) + mm_tanh(C(0.79788456080286535588) * (x + C(0.044715) * x * x * x)));
+		case ACT_GELU_TANH: return C(0.5) * x * (C(1) + F::tanh_of(C(0.79788456080286535588) * (x + C(0.044715) * x * x * x)));
 		case ACT_RELU: return x < C(0) ? C(0) : x; // (a NaN stays one)
 		default: return x;
 	}
 }
-template <class C>
-__device__ __forceinline__ C mm_act_slope(C x, int act) {
+// value and derivative
+template <class T, class C>
+__device__ __forceinline__ void mm_act_both(C x, int act, C& value, C& slope) {
+	typedef MmMath<T> F;
 	switch(act) {
-		case ACT_SIGMOID: { const C s = C(1) / (C(1) + mm_exp(-x)); return s * (C(1) - s); }
-		case ACT_SILU: { const C s = C(1) / (C(1) + mm_exp(-x)); return s * (C(1) + x * (C(1) - s)); }
-		case ACT_GELU: return C(0.5) * (C(1) + mm_erf(x * C(0.70710678118654752440))) + x * mm_exp(C(-0.5) * x * x) * C(0.39894228040143267794);
-		case ACT_GELU_TANH: {
-			const C c = C(0.79788456080286535588), t = mm_tanh(c * (x + C(0.044715) * x * x * x));
-			return C(0.5) * (C(1) + t) + C(0.5) * x * (C(1) - t * t) * c * (C(1) + C(0.134145) * x * x);
+		case ACT_SIGMOID: { value = F::logistic(x); slope = value * (C(1) - value); break; }
+		case ACT_SILU: { const C s = F::logistic(x); value = x * s; slope = s * (C(1) + x * (C(1) - s)); break; }
+		case ACT_GELU: {
+			const C p = C(0.5) * (C(1) + mm_erf(x * C(0.70710678118654752440)));
+			value = x * p; slope = p + x * F::gauss(x) * C(0.39894228040143267794);
+			break;
 		}
-		case ACT_RELU: return x > C(0) ? C(1) : C(0);
-		default: return C(1);
+		case ACT_GELU_TANH: {
+			const C c = C(0.79788456080286535588), t = F::tanh_of(c * (x + C(0.044715) * x * x * x));
+			value = C(0.5) * x * (C(1) + t);
+			slope = C(0.5) * (C(1) + t) + C(0.5) * x * (C(1) - t * t) * c * (C(1) + C(0.134145) * x * x);
+			break;
+		}
+		case ACT_RELU: { value = x < C(0) ? C(0) : x; slope = x > C(0) ? C(1) : C(0); break; }
+		default: { value = x; slope = C(1); break; }
 	}
 }
 
@@ -219,8 +242,9 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN / (WM * WN) >= 128 * 128 ? 1 
 	const char* const pUp = GATED ? pCols + (int64_t) A.N * A.ldCols : pCols;
 	const int ldR = (int) A.ldRows, ldC = (int) A.ldCols; // (at most MM_MAX_LD, or 2^31 - 1 where offsets are not held in 32 bits)
 
-	// a wave takes every NW-th 8 rows of the tile; lane: row lane / 8 of them, piece (lane % 8) ^ (lane / 8) of the step
-	const int lr = lane >> 3, piece = ((lane & 7) ^ lr) * 16;
+	// a wave takes every NW-th 8 rows of the tile; lane: row lane / 8 of them, the piece of the step that belongs at place lane % 8
+	static_assert(NW % 2 == 0, "a wave's rows / 2 are alike modulo 8");
+	const int lr = lane >> 3, piece = ((lane & 7) ^ (((wave & 1) << 2) + (lr >> 1))) * 16;
 	auto col_half = [&](int i) { return GATED ? ((i * 8) / FR) & 1 : 0; };                     // gate's or the other projection's
 	auto col_row = [&](int i) { return GATED ? ((i * 8) / (2 * FR)) * FR + (i * 8) % FR : i * 8; }; // first of 8 columns
 	__amdgpu_buffer_rsrc_t rRows, rCols, rUp;
@@ -280,7 +304,7 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN / (WM * WN) >= 128 * 128 ? 1 
 	mm_i32x4 fc[2][NF], fr[2][MF];
 	const int fl = (lane % FR) * 128;
 	auto read = [&](int set, int t, int s) {
-		const char* const from = mm_smem + (t & 1) * BUF + fl + (((s * PIECES + lane / FR) ^ (lane & 7)) << 4);
+		const char* const from = mm_smem + (t & 1) * BUF + fl + (((s * PIECES + lane / FR) ^ ((lane % FR >> 1) & 7)) << 4);
 #pragma unroll
 		for(int j = 0; j < MF; j++) fr[set][j] = *(const mm_i32x4*) (from + (wm * SM + j * FR) * 128);
 #pragma unroll

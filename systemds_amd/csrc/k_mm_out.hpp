@@ -71,30 +71,42 @@ template <class T, bool SCALED> struct MmEpiOut {
 		typedef typename MmCalc<T>::type C;
 		constexpr int FR = Reg::FR, H = Reg::H, V = 16 / (int) sizeof(T), PER = Reg::COLS / V;
 		static_assert(Reg::COLS % V == 0, "a row of the region is whole stores");
-		const int cols = N - n0;
+		static_assert(64 % PER == 0 && FR * PER % 64 == 0, "a lane keeps its columns");
+		// a lane's columns are the same ones in every row: their scales and biases stay in registers; the scales of the wave's rows are held one by a lane
+		const int c = (lane % PER) * V, cols = N - n0 - c;
+		C sc[H][V], bi[H][V];
+		float sr[(MF * FR + 63) / 64];
+#pragma unroll
+		for(int h = 0; h < H; h++)
+#pragma unroll
+			for(int v = 0; v < V; v++) {
+				const int col = min(n0 + c + v, N - 1) + h * N;
+				sc[h][v] = SCALED ? (C) sCol[col] : C(1);
+				bi[h][v] = bias ? (C) bias[col] : C(0);
+			}
+#pragma unroll
+		for(int i = 0; i < (MF * FR + 63) / 64; i++) sr[i] = SCALED ? sRow[min(m0 + i * 64 + lane, M - 1)] : 1.0f;
 #pragma unroll
 		for(int j = 0; j < MF; j++) {
 			Reg::template put<MF>(region, acc, j, lane);
 			const int64_t row0 = m0 + j * FR;
 #pragma unroll 1
-			for(int i = lane; i < FR * PER; i += 64) {
-				const int r = i / PER, c = (i % PER) * V;
-				if(row0 + r >= M || c >= cols) continue;
-				const float sr = SCALED ? sRow[row0 + r] : 1.0f;
+			for(int r0 = 0; r0 < FR; r0 += 64 / PER) {
+				const int r = r0 + lane / PER;
+				const C s = SCALED ? (C) __shfl(sr[j * FR / 64], (j * FR + r) & 63, 64) : C(1);
 				T x[V];
 #pragma unroll
 				for(int v = 0; v < V; v++) {
-					const int col = min(n0 + c + v, N - 1);
 					C y[H];
 #pragma unroll
 					for(int h = 0; h < H; h++) {
 						y[h] = (C) Reg::at(region, h, r, c)[v];
-						if(SCALED) y[h] *= (C) sr * (C) sCol[col + h * N];
-						if(bias) y[h] += (C) bias[col + h * N];
+						if(SCALED) y[h] *= s * sc[h][v];
+						y[h] += bi[h][v];
 					}
-					x[v] = (T) (GATED ? mm_act<C>(y[0], act) * y[H - 1] : y[0]);
+					x[v] = (T) (GATED ? mm_act<T>(y[0], act) * y[H - 1] : y[0]);
 				}
-				mm_store<T, V>(out + part * zOut + (row0 + r) * ld + n0 + c, x, cols - c, aligned);
+				if(row0 + r < M && cols > 0) mm_store<T, V>(out + part * zOut + (row0 + r) * ld + n0 + c, x, cols, aligned);
 			}
 			mm_wave_sync();
 		}
@@ -123,40 +135,45 @@ template <class T> struct MmEpiBack {
 		typedef MmRegion<E, NF, GATED> Reg;
 		constexpr int FR = Reg::FR, COLS = Reg::COLS, V = 16 / (int) sizeof(T), PER = COLS / V, S = (2 * COLS + 63) / 64;
 		static_assert(GATED && COLS % V == 0 && FR % V == 0, "two halves, whole stores both ways");
-		const int cols = N - n0, half = (int) (ldP / 2) - n0;
-		C sum[S];
+		static_assert(64 % PER == 0 && FR * PER % 64 == 0, "a lane keeps its columns");
+		const int c0 = (lane % PER) * V, cols = N - n0, half = (int) (ldP / 2) - n0;
+		C sum[S], bg[V], bu[V];
 #pragma unroll
 		for(int s = 0; s < S; s++) sum[s] = C(0);
+#pragma unroll
+		for(int v = 0; v < V; v++) {
+			const int col = min(n0 + c0 + v, N - 1);
+			bg[v] = bias ? (C) bias[col] : C(0);
+			bu[v] = bias ? (C) bias[col + N] : C(0);
+		}
 #pragma unroll
 		for(int j = 0; j < MF; j++) {
 			Reg::template put<MF>(region, acc, j, lane);
 			const int64_t row0 = m0 + j * FR;
 #pragma unroll 1
-			for(int i = lane; i < FR * PER; i += 64) {
-				const int r = i / PER, c = (i % PER) * V;
-				const bool in = row0 + r < M && c < cols;
-				const T* const d = D + (row0 + r) * ldD + n0 + c;
+			for(int r0 = 0; r0 < FR; r0 += 64 / PER) {
+				const int r = r0 + lane / PER;
+				const bool in = row0 + r < M && c0 < cols;
+				const T* const d = D + (row0 + r) * ldD + n0 + c0;
 				T g[V], u[V];
 				MmPack<T, V> dv;
-				if(in && alignedD && c + V <= cols) dv = *(const MmPack<T, V>*) d;
+				if(in && alignedD && c0 + V <= cols) dv = *(const MmPack<T, V>*) d;
 				else {
 #pragma unroll
-					for(int v = 0; v < V; v++) dv.x[v] = in && c + v < cols ? d[v] : (T) 0.0f;
+					for(int v = 0; v < V; v++) dv.x[v] = in && c0 + v < cols ? d[v] : (T) 0.0f;
 				}
 #pragma unroll
 				for(int v = 0; v < V; v++) {
-					C x = *Reg::at(region, 0, r, c + v), y = *Reg::at(region, 1, r, c + v);
-					if(bias) {
-						const int col = min(n0 + c + v, N - 1);
-						x += (C) bias[col]; y += (C) bias[col + N];
-					}
-					const bool there = in && c + v < cols;
-					const C dG = there ? (C) dv.x[v] * y * mm_act_slope<C>(x, act) : C(0), dU = there ? (C) dv.x[v] * mm_act<C>(x, act) : C(0);
-					*Reg::at(region, 0, r, c + v) = dG; *Reg::at(region, 1, r, c + v) = dU;
+					const C x = *Reg::at(region, 0, r, c0 + v) + bg[v], y = *Reg::at(region, 1, r, c0 + v) + bu[v];
+					C value, slope;
+					mm_act_both<T>(x, act, value, slope);
+					const bool there = in && c0 + v < cols;
+					const C dG = there ? (C) dv.x[v] * y * slope : C(0), dU = there ? (C) dv.x[v] * value : C(0);
+					*Reg::at(region, 0, r, c0 + v) = dG; *Reg::at(region, 1, r, c0 + v) = dU;
 					g[v] = (T) dG; u[v] = (T) dU;
 				}
-				if(P && row0 + r < M && c < half) {
-					T* const to = P + (row0 + r) * ldP + n0 + c;
+				if(P && row0 + r < M && c0 < half) {
+					T* const to = P + (row0 + r) * ldP + n0 + c0;
 					mm_store<T, V>(to, g, V, true);
 					mm_store<T, V>(to + ldP / 2, u, V, true);
 				}

@@ -247,7 +247,7 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_q8_few(Q8Few<T> A) {
 			x[h] = (C) sum * ((C) A.s[row] * (C) A.t[col + h * A.N]);
 			if(A.bias) x[h] += (C) A.bias[col + h * A.N];
 		}
-		A.out[row * A.ld + col] = (T) (GATED ? mm_act<C>(x[0], A.act) * x[H - 1] : x[0]);
+		A.out[row * A.ld + col] = (T) (GATED ? mm_act<T>(x[0], A.act) * x[H - 1] : x[0]);
 	}
 }
 
