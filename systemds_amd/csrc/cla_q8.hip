@@ -80,12 +80,13 @@ struct DevTmp { // device memory of a call that waits
 };
 
 static int product(cla_q8* h, const char* what, bool gated, int act, const int8_t* Q, int64_t ldQ, const float* s, int64_t m, const void* bias, void* out, int type,
-	int64_t ldOut) {
+	int64_t ldOut, const void* Y = nullptr, int64_t ldY = 0) {
 	Q8Product p{};
 	p.W = h->dW; p.ldW = h->ldW; p.t = h->dScale;
 	p.Q = Q; p.ldQ = ldQ; p.s = s; p.m = m;
 	p.K = (int32_t) h->nRows; p.N = h->nCols; p.act = act;
 	p.bias = bias; p.out = out; p.ldOut = ldOut;
+	p.Y = Y; p.ldY = ldY;
 	const int64_t n = h->nCols; // (tiles of the smallest shape)
 	if(((m + 63) / 64) * ((n + 63) / 64) > 0x7fffffffLL) { set_error("%s: %lld x %lld outputs", what, (long long) m, (long long) n); return -CLA_ERR_UNSUPPORTED; }
 	return launch_q8(p, type, gated, h->stream);
@@ -114,6 +115,7 @@ static int from_rows(cla_q8* h, const char* what, bool gated, int act, const voi
 		return -CLA_ERR_INVALID;
 	}
 	std::lock_guard<std::recursive_mutex> lk(h->mu);
+	if(q8_fuses(m, h->nRows)) return product(h, what, gated, act, nullptr, 0, nullptr, m, dBias, dOut, type, ldOut, dY, ldY);
 	float* const s = (float*) ws;
 	int8_t* const q = (int8_t*) ws + up((size_t) m * sizeof(float), 256);
 	const int64_t ldQ = ld_rows(h);

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_gate_few(GateFew<T> A) {
 	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
 	Acc acc[2][MR];
 	auto rowOf = [&](int row, int64_t k, int64_t left) { return mm_load16<sizeof(T)>((const char*) (A.Y + (row < A.m ? row : 0) * A.ldY) + k, row < A.m ? left : 0); };
-	mm_few<T, true, MR>((const char*) A.W, A.ldW * (int64_t) sizeof(T), n0, A.nOut, (int64_t) A.nIn * sizeof(T), rowOf, acc, wave, lane);
+	mm_few<T, true, MR>((const char*) A.W, A.ldW * (int64_t) sizeof(T), n0, A.nOut, (int64_t) A.nIn * sizeof(T), rowOf, [] {}, acc, wave, lane);
 	C* const red = (C*) gate_smem;
 #pragma unroll
 	for(int h = 0; h < 2; h++)

@@ -168,7 +168,7 @@ template <int ES>
 __device__ __forceinline__ mm_i32x4 mm_load16(const char* p, int64_t left) {
 	mm_i32x4 v = {0, 0, 0, 0};
 	if(left >= 16) __builtin_memcpy(&v, p, 16);
-	else if(left > 0) {
+	if(left > 0 && left < 16) { // (rare: behind a branch of its own, so that a lane's next loads do not wait for it)
 		if(ES == 8) { // (one of two)
 			uint64_t x;
 			__builtin_memcpy(&x, p, 8);
@@ -360,37 +360,54 @@ __global__ __launch_bounds__(64 * WM * WN, TM * TN / (WM * WN) >= 128 * 128 ? 1 
 
 // The same for few rows (up to 16 MR): columns are a stream of bytes that is read once, from global memory straight into the matrix operand. A block
 // takes 16 columns (gated: of either projection), its waves take turns of the summed index and add their sums up in LDS, in the order of the waves.
-// Lane: column (and row) lane % 16, 16 bytes from 16 (lane / 16) on of every 64. Rows that are not there are zeros.
+// Lane: column (and row) lane % 16, 16 bytes from 16 (lane / 16) on of every 64. Rows that are not there are zeros. A turn's columns are requested a turn
+// ahead, the first ones in front of `before` (what has to be done before rowOf gives rows).
 constexpr int MMF_WAVES = 8, MMF_UNROLL = 4;
-template <class E, bool GATED, int MR, class Rows>
-__device__ __forceinline__ void mm_few(const char* cols, int64_t ldCols, int n0, int N, int64_t K, const Rows& rowOf, typename MmOp<E>::Acc16 (&acc)[GATED ? 2 : 1][MR],
-	int wave, int lane) {
+template <class E, bool GATED, int MR, class Rows, class Before>
+__device__ __forceinline__ void mm_few(const char* cols, int64_t ldCols, int n0, int N, int64_t K, const Rows& rowOf, const Before& before,
+	typename MmOp<E>::Acc16 (&acc)[GATED ? 2 : 1][MR], int wave, int lane) {
 	typedef MmOp<E> Op;
-	constexpr int H = GATED ? 2 : 1;
+	constexpr int H = GATED ? 2 : 1, U = MMF_UNROLL;
+	constexpr int64_t TURN = 64 * U, STEP = MMF_WAVES * TURN;
 	const int l16 = lane & 15;
 	const int64_t at = (lane >> 4) * 16;
 	const int c = min(n0 + l16, N - 1);
-	const char* const p[2] = {cols + (int64_t) c * ldCols, cols + ((int64_t) c + (GATED ? N : 0)) * ldCols};
+	const char* const p[2] = {cols + (int64_t) c * ldCols + at, cols + ((int64_t) c + (GATED ? N : 0)) * ldCols + at};
+	mm_i32x4 w[2][H][U];
+	auto load = [&](int set, int64_t k) {
+#pragma unroll
+		for(int u = 0; u < U; u++)
+#pragma unroll
+			for(int h = 0; h < H; h++) w[set][h][u] = mm_load16<sizeof(E)>(p[h] + k + u * 64, K - (k + u * 64 + at));
+	};
+	auto multiply = [&](int set, int64_t k) {
+		mm_i32x4 y[MR][U];
+#pragma unroll
+		for(int u = 0; u < U; u++)
+#pragma unroll
+			for(int j = 0; j < MR; j++) y[j][u] = rowOf(16 * j + l16, k + u * 64 + at, K - (k + u * 64 + at));
+#pragma unroll
+		for(int u = 0; u < U; u++)
+#pragma unroll
+			for(int h = 0; h < H; h++)
+#pragma unroll
+				for(int j = 0; j < MR; j++) Op::mma16(acc[h][j], w[set][h][u], y[j][u]);
+	};
 #pragma unroll
 	for(int h = 0; h < H; h++)
 #pragma unroll
 		for(int j = 0; j < MR; j++) acc[h][j] = typename Op::Acc16{0, 0, 0, 0};
-	for(int64_t k = (int64_t) wave * 64 * MMF_UNROLL; k < K; k += MMF_WAVES * 64 * MMF_UNROLL) {
-		mm_i32x4 w[H][MMF_UNROLL], y[MR][MMF_UNROLL];
-#pragma unroll
-		for(int u = 0; u < MMF_UNROLL; u++)
-#pragma unroll
-			for(int h = 0; h < H; h++) w[h][u] = mm_load16<sizeof(E)>(p[h] + k + u * 64 + at, K - (k + u * 64 + at));
-#pragma unroll
-		for(int u = 0; u < MMF_UNROLL; u++)
-#pragma unroll
-			for(int j = 0; j < MR; j++) y[j][u] = rowOf(16 * j + l16, k + u * 64 + at, K - (k + u * 64 + at));
-#pragma unroll
-		for(int u = 0; u < MMF_UNROLL; u++)
-#pragma unroll
-			for(int h = 0; h < H; h++)
-#pragma unroll
-				for(int j = 0; j < MR; j++) Op::mma16(acc[h][j], w[h][u], y[j][u]);
+	int64_t k = wave * TURN;
+	if(k < K) load(0, k);
+	before();
+	while(k < K) { // (uniform)
+		if(k + STEP < K) load(1, k + STEP);
+		multiply(0, k);
+		k += STEP;
+		if(k >= K) break;
+		if(k + STEP < K) load(0, k + STEP);
+		multiply(1, k);
+		k += STEP;
 	}
 }
 

@@ -15,90 +15,64 @@ namespace cla {
 template <class T> struct Q8Most { static __device__ __forceinline__ float value() { return 3.4028234663852886e38f; } };
 template <> struct Q8Most<double> { static __device__ __forceinline__ double value() { return 1.7976931348623157e308; } };
 
-// 8 neighbouring values of a row, `left` of them there (the others 0)
-template <class T>
-__device__ __forceinline__ void q8_load(const T* p, int64_t left, typename MmCalc<T>::type (&x)[8]) {
+// 16 bytes of a row (V values), `left` values of them there (the others 0)
+template <class T> struct Q8Piece {
+	static constexpr int V = 16 / (int) sizeof(T);
 	typedef typename MmCalc<T>::type C;
-	if(left >= 8) {
-		T v[8];
-		__builtin_memcpy(v, p, sizeof(v));
+	static __device__ __forceinline__ mm_i32x4 load(const T* p, int64_t left) { return mm_load16<sizeof(T)>((const char*) p, left * (int) sizeof(T)); }
+	static __device__ __forceinline__ C value(const mm_i32x4& p, int v) { return (C) __builtin_bit_cast(Vals, p).x[v]; }
+	struct Vals { T x[V]; };
+	// largest magnitude; infinity where a value is none (infinite or NaN)
+	static __device__ __forceinline__ C largest(const mm_i32x4& p, C m) {
 #pragma unroll
-		for(int i = 0; i < 8; i++) x[i] = (C) v[i];
+		for(int v = 0; v < V; v++) {
+			const C a = fabs(value(p, v));
+			m = a <= Q8Most<C>::value() ? (a > m ? a : m) : (C) INFINITY;
+		}
+		return m;
 	}
-	else {
-#pragma unroll
-		for(int i = 0; i < 8; i++) x[i] = i < left ? (C) p[i] : C(0);
-	}
-}
+};
 
-// Largest magnitude; infinity where a value is none (infinite or NaN).
-template <class C>
-__device__ __forceinline__ C q8_largest(const C (&x)[8], C m) {
-#pragma unroll
-	for(int i = 0; i < 8; i++) {
-		const C a = fabs(x[i]);
-		m = a <= Q8Most<C>::value() ? (a > m ? a : m) : (C) INFINITY;
-	}
-	return m;
-}
-
-// The scale of a row: the largest times 1 / 127, both in fp32. A row with a value that is not finite, or whose largest is none in fp32, has the scale NaN (and zeros): its outputs are NaN.
+// The scale of a row: the largest times 1 / 127, both in fp32. A row with a value that is not finite, or whose largest is none in fp32, has the scale NaN (and
+// zeros): its outputs are NaN.
 template <class C>
 __device__ __forceinline__ float q8_scale(C largest) {
 	const float a = (float) largest;
 	return a <= 3.4028234663852886e38f ? a * (1.0f / 127.0f) : NAN;
 }
 
-// x / s to the nearest whole number, ties to even, as the exact quotient rounds. fp32: the product with the reciprocal is within one of it; x - r s is exact in
-// fp32 next to s / 2 (both are multiples of half of s's last place, and below 2^24 of those), so comparing it with s / 2 decides. Scales whose reciprocal or
-// last place leaves fp32's range take the fp64 quotient, whose distance from a half no fp32 operands can lose.
-__device__ __forceinline__ int q8_round(float x, float s, float inv) {
-	float r = rintf(x * inv);
-	const float d = fmaf(-r, s, x), half = 0.5f * s;
-	if(d > half || (d == half && ((int) r & 1))) r += 1.0f;
-	else if(d < -half || (d == -half && ((int) r & 1))) r -= 1.0f;
-	return (int) fminf(fmaxf(r, -127.0f), 127.0f);
-}
-__device__ __forceinline__ int q8_round_wide(double x, double s) { return (int) fmin(fmax(rint(x / s), -127.0), 127.0); }
-
+// x / s to the nearest whole number, ties to even, as the exact quotient rounds: the product with the reciprocal is within one of it, and x - r s is exact next to
+// s / 2 (both are multiples of x's or half of s's last place, below 2^24 or 2^53 of those), so comparing it with s / 2 decides. Scales whose reciprocal or
+// last place leaves the range take the quotient in fp64, whose distance from a half no fp32 operands can lose.
 template <class C>
-__device__ __forceinline__ uint64_t q8_pack(const C (&x)[8], float s) {
-	uint64_t v = 0;
-	if(!(s > 0.0f)) return 0; // a row of zeros, or one with the scale NaN
-	if(std::is_same<C, double>::value || s < 1e-30f) {
-#pragma unroll
-		for(int i = 0; i < 8; i++) v |= (uint64_t) (uint8_t) q8_round_wide((double) x[i], (double) s) << (8 * i);
-	}
-	else {
-		const float inv = 1.0f / s;
-#pragma unroll
-		for(int i = 0; i < 8; i++) v |= (uint64_t) (uint8_t) q8_round((float) x[i], s, inv) << (8 * i);
-	}
-	return v;
+__device__ __forceinline__ int q8_round(C x, C s, C inv) {
+	C r = rint(x * inv);
+	const C d = fma(-r, s, x), half = C(0.5) * s;
+	const bool odd = ((int) r & 1) != 0;
+	if(d > half || (d == half && odd)) r += C(1);
+	else if(d < -half || (d == -half && odd)) r -= C(1);
+	return (int) fmin(fmax(r, C(-127)), C(127));
 }
+template <class C>
+__device__ __forceinline__ int q8_round_wide(C x, float s) { return (int) fmin(fmax(rint((double) x / (double) s), -127.0), 127.0); }
 
-// TPR threads to a row; what a thread holds of it (32 values) stays in registers between the search for the largest and the rounding, longer rows are read
-// again. Bound: a row's bytes in and a quarter to a half of them out.
-template <class T, int TPR>
+// TPR threads to a row, NV pieces each, which stay in registers between the search for the largest and the rounding; longer rows are read again. Bound: a
+// row's bytes in and an eighth to a half of them out.
+template <class T, int TPR, int NV>
 __global__ __launch_bounds__(256) void k_q8_rows(const T* __restrict__ Y, int64_t m, int K, int64_t ld, int8_t* __restrict__ Q, int64_t ldQ, float* __restrict__ scale) {
-	typedef typename MmCalc<T>::type C;
-	constexpr int NV = 4;
+	typedef Q8Piece<T> P;
+	typedef typename P::C C;
+	constexpr int V = P::V;
 	const int t = threadIdx.x % TPR;
-	const int64_t row = (int64_t) blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
-	if(TPR <= 64 && row >= m) return; // (TPR 256: the grid has m blocks)
-	const T* const y = Y + row * ld;
-	C x[NV][8], largest = C(0);
+	const int64_t row = (int64_t) blockIdx.x * (256 / TPR) + threadIdx.x / TPR, at = min(row, m - 1); // (threads behind the last row follow it and write nothing)
+	const T* const y = Y + at * ld;
+	mm_i32x4 x[NV];
 #pragma unroll
-	for(int i = 0; i < NV; i++) {
-		const int k = (i * TPR + t) * 8;
-		q8_load<T>(y + k, K - k, x[i]);
-		largest = q8_largest<C>(x[i], largest);
-	}
-	for(int k = (NV * TPR + t) * 8; k < K; k += TPR * 8) {
-		C z[8];
-		q8_load<T>(y + k, K - k, z);
-		largest = q8_largest<C>(z, largest);
-	}
+	for(int i = 0; i < NV; i++) x[i] = P::load(y + (i * TPR + t) * V, K - (i * TPR + t) * V);
+	C largest = C(0);
+#pragma unroll
+	for(int i = 0; i < NV; i++) largest = P::largest(x[i], largest);
+	for(int k = (NV * TPR + t) * V; k < K; k += TPR * V) largest = P::largest(P::load(y + k, K - k), largest);
 #pragma unroll
 	for(int d = (TPR < 64 ? TPR : 64) / 2; d > 0; d >>= 1) {
 		const C o = __shfl_xor(largest, d, 64);
@@ -111,30 +85,46 @@ __global__ __launch_bounds__(256) void k_q8_rows(const T* __restrict__ Y, int64_
 #pragma unroll
 		for(int i = 0; i < 4; i++) largest = part[i] > largest ? part[i] : largest;
 	}
+	if(row >= m) return;
 	const float s = q8_scale<C>(largest);
 	if(t == 0) scale[row] = s;
 	int8_t* const q = Q + row * ldQ;
-	auto put = [&](int k, const C (&z)[8]) {
-		const uint64_t v = q8_pack<C>(z, s);
-		if(k + 8 <= K && (((uintptr_t) q | (uintptr_t) ldQ) & 7) == 0) *(uint64_t*) (q + k) = v;
-		else
-			for(int i = 0; i < 8 && k + i < K; i++) q[k + i] = (int8_t) (v >> (8 * i));
+	const bool whole = (((uintptr_t) Q | (uintptr_t) ldQ) & (V - 1)) == 0, none = !(s > 0.0f), wide = s < 1e-30f;
+	const C inv = C(1) / (C) s;
+	auto put = [&](int k, const mm_i32x4& p) {
+		MmPack<int8_t, V> o;
+#pragma unroll
+		for(int v = 0; v < V; v++) o.x[v] = (int8_t) (none ? 0 : wide ? q8_round_wide<C>(P::value(p, v), s) : q8_round<C>(P::value(p, v), (C) s, inv));
+		if(whole && k + V <= K) *(MmPack<int8_t, V>*) (q + k) = o;
+		else {
+#pragma unroll
+			for(int v = 0; v < V; v++)
+				if(k + v < K) q[k + v] = o.x[v];
+		}
 	};
 #pragma unroll
-	for(int i = 0; i < NV; i++) put((i * TPR + t) * 8, x[i]);
-	for(int k = (NV * TPR + t) * 8; k < K; k += TPR * 8) {
-		C z[8];
-		q8_load<T>(y + k, K - k, z);
-		put(k, z);
-	}
+	for(int i = 0; i < NV; i++)
+		if(i * TPR * V < K) put((i * TPR + t) * V, x[i]);
+	for(int k = (NV * TPR + t) * V; k < K; k += TPR * V) put(k, P::load(y + k, K - k));
 }
 
 template <class T>
-static int q8_rows(const void* Y, int64_t m, int K, int64_t ld, int8_t* Q, int64_t ldQ, float* scale, hipStream_t stream) {
+static int q8_rows(const void* Yp, int64_t m, int K, int64_t ld, int8_t* Q, int64_t ldQ, float* scale, hipStream_t stream) {
 	if(m == 0) return 0;
-	// up to 2048 values a wave holds a row in its registers (four rows to a block), beyond that a block does
-	if(K <= 2048) k_q8_rows<T, 64><<<(unsigned) ((m + 3) / 4), 256, 0, stream>>>((const T*) Y, m, K, ld, Q, ldQ, scale);
-	else k_q8_rows<T, 256><<<(unsigned) m, 256, 0, stream>>>((const T*) Y, m, K, ld, Q, ldQ, scale);
+	constexpr int V = 16 / (int) sizeof(T);
+	const T* const Y = (const T*) Yp;
+	// Short rows 16 threads each, 16 rows a block; up to 8 pieces a lane a wave holds the row and no barrier is needed.
+	const int64_t pieces = (K + V - 1) / V;
+#define Q8_ROWS(TPR, NV) k_q8_rows<T, TPR, NV><<<(unsigned) ((m + 256 / TPR - 1) / (256 / TPR)), 256, 0, stream>>>(Y, m, K, ld, Q, ldQ, scale)
+	if(pieces <= 16) Q8_ROWS(16, 1);
+	else if(pieces <= 64) Q8_ROWS(16, 4);
+	else if(m < 1024 || pieces > 64 * 8) {
+		if(pieces <= 512) Q8_ROWS(256, 2);
+		else Q8_ROWS(256, 8);
+	}
+	else if(pieces <= 64 * 2) Q8_ROWS(64, 2);
+	else Q8_ROWS(64, 8);
+#undef Q8_ROWS
 	CLA_HIP(hipGetLastError());
 	return 0;
 }
@@ -215,19 +205,78 @@ template <class T> struct Q8Few {
 	const T* bias;
 	T* out;
 	int64_t ld;
+	const T* Y;         // FUSE: rows as they come, in place of Q and s
+	int64_t ldY;
 };
 
-template <class T, bool GATED, int MR>
+// FUSE: each block quantises the rows itself, into LDS, while its first weights are on their way: up to Q8_FUSE rows that costs less than a kernel in front.
+constexpr int Q8_FUSE = 4, Q8_FUSE_LDS = 64 << 10;
+
+template <class T, bool GATED, int MR, bool FUSE>
 __global__ __launch_bounds__(64 * MMF_WAVES) void k_q8_few(Q8Few<T> A) {
-	extern __shared__ __attribute__((aligned(16))) char q8_smem[]; // sums: [wave][half][row][column]
+	extern __shared__ __attribute__((aligned(16))) char q8_smem[]; // sums: [wave][half][row][column]; FUSE: the 8-bit rows behind them
 	typedef typename MmCalc<T>::type C;
-	constexpr int H = GATED ? 2 : 1;
-	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
+	constexpr int H = GATED ? 2 : 1, SUMS = MMF_WAVES * H * MR * 1024;
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = blockIdx.x * 16;
+	__shared__ float scales[FUSE ? Q8_FUSE : 1];
 	mm_i32x4 acc[H][MR];
-	auto rowOf = [&](int row, int64_t k, int64_t) {
-		return row < A.m && k < A.K ? *(const mm_i32x4*) (A.Q + row * A.ldQ + k) : mm_i32x4{0, 0, 0, 0};
+	const int pitch = (A.K + 15) & ~15;
+	auto quantise = [&]() {
+		if constexpr(FUSE) {
+			typedef Q8Piece<T> P;
+			constexpr int V = P::V, NV = 2, NT = 64 * MMF_WAVES;
+			__shared__ C part[Q8_FUSE][MMF_WAVES];
+			mm_i32x4 x[Q8_FUSE][NV];
+#pragma unroll
+			for(int r = 0; r < Q8_FUSE; r++)
+#pragma unroll
+				for(int i = 0; i < NV; i++) x[r][i] = P::load(A.Y + min(r, A.m - 1) * A.ldY + (i * NT + tid) * V, r < A.m ? A.K - (i * NT + tid) * V : 0);
+			C big[Q8_FUSE];
+#pragma unroll
+			for(int r = 0; r < Q8_FUSE; r++) {
+				big[r] = C(0);
+#pragma unroll
+				for(int i = 0; i < NV; i++) big[r] = P::largest(x[r][i], big[r]);
+				if(r < A.m)
+					for(int k = (NV * NT + tid) * V; k < A.K; k += NT * V) big[r] = P::largest(P::load(A.Y + r * A.ldY + k, A.K - k), big[r]);
+#pragma unroll
+				for(int d = 32; d > 0; d >>= 1) {
+					const C o = __shfl_xor(big[r], d, 64);
+					big[r] = o > big[r] ? o : big[r];
+				}
+				if(lane == 0) part[r][wave] = big[r];
+			}
+			__syncthreads();
+#pragma unroll
+			for(int r = 0; r < Q8_FUSE; r++) {
+				if(r >= A.m) break;
+				C most = part[r][0];
+#pragma unroll
+				for(int w = 1; w < MMF_WAVES; w++) most = part[r][w] > most ? part[r][w] : most;
+				const float s = q8_scale<C>(most);
+				if(tid == 0) scales[r] = s;
+				const bool none = !(s > 0.0f), wide = s < 1e-30f;
+				const C inv = C(1) / (C) s;
+				auto put = [&](int k, const mm_i32x4& p) { // (what lies behind the row is 0: so are the piece's bytes)
+					MmPack<int8_t, V> o;
+#pragma unroll
+					for(int v = 0; v < V; v++) o.x[v] = (int8_t) (none ? 0 : wide ? q8_round_wide<C>(P::value(p, v), s) : q8_round<C>(P::value(p, v), (C) s, inv));
+					*(MmPack<int8_t, V>*) (q8_smem + SUMS + r * pitch + k) = o;
+				};
+#pragma unroll
+				for(int i = 0; i < NV; i++)
+					if((i * NT + tid) * V < pitch) put((i * NT + tid) * V, x[r][i]);
+				for(int k = (NV * NT + tid) * V; k < pitch; k += NT * V) put(k, P::load(A.Y + r * A.ldY + k, A.K - k));
+			}
+			__syncthreads();
+		}
 	};
-	mm_few<int8_t, GATED, MR>((const char*) A.W, A.ldW, n0, A.N, A.ldW, rowOf, acc, wave, lane);
+	auto rowOf = [&](int row, int64_t k, int64_t) {
+		const bool in = row < A.m && k < A.K;
+		if(FUSE) return in ? *(const mm_i32x4*) (q8_smem + SUMS + row * pitch + k) : mm_i32x4{0, 0, 0, 0};
+		return in ? *(const mm_i32x4*) (A.Q + row * A.ldQ + k) : mm_i32x4{0, 0, 0, 0};
+	};
+	mm_few<int8_t, GATED, MR>((const char*) A.W, A.ldW, n0, A.N, A.ldW, rowOf, quantise, acc, wave, lane);
 	int* const red = (int*) q8_smem;
 #pragma unroll
 	for(int h = 0; h < H; h++)
@@ -235,16 +284,17 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_q8_few(Q8Few<T> A) {
 		for(int j = 0; j < MR; j++)
 			*(mm_i32x4*) (red + (((wave * H + h) * MR * 16) + 16 * j + (lane & 15)) * 16 + 4 * (lane >> 4)) = acc[h][j];
 	__syncthreads();
-	for(int i = threadIdx.x; i < A.m * 16; i += 64 * MMF_WAVES) {
+	for(int i = tid; i < A.m * 16; i += 64 * MMF_WAVES) {
 		const int row = i >> 4, col = n0 + (i & 15);
 		if(col >= A.N) continue;
+		const float s = FUSE ? scales[FUSE ? row : 0] : A.s[row];
 		C x[H];
 #pragma unroll
 		for(int h = 0; h < H; h++) {
 			int sum = 0;
 #pragma unroll
 			for(int w = 0; w < MMF_WAVES; w++) sum += red[(w * H + h) * MR * 256 + i];
-			x[h] = (C) sum * ((C) A.s[row] * (C) A.t[col + h * A.N]);
+			x[h] = (C) sum * ((C) s * (C) A.t[col + h * A.N]);
 			if(A.bias) x[h] += (C) A.bias[col + h * A.N];
 		}
 		A.out[row * A.ld + col] = (T) (GATED ? mm_act<T>(x[0], A.act) * x[H - 1] : x[0]);
@@ -255,10 +305,18 @@ template <class T, bool GATED>
 static int q8_few(const Q8Few<T>& A, hipStream_t stream) {
 	const unsigned grid = (unsigned) ((A.N + 15) / 16);
 	const int MR = A.m <= 16 ? 1 : A.m <= 32 ? 2 : 4;
-	const size_t lds = (size_t) MMF_WAVES * (GATED ? 2 : 1) * MR * 1024;
-	if(MR == 1) k_q8_few<T, GATED, 1><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
-	else if(MR == 2) k_q8_few<T, GATED, 2><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
-	else k_q8_few<T, GATED, 4><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
+	size_t lds = (size_t) MMF_WAVES * (GATED ? 2 : 1) * MR * 1024;
+	if(A.Y) {
+		lds += (size_t) A.m * ((A.K + 15) & ~15);
+		CLA_HIP(allow_full_lds((const void*) k_q8_few<T, GATED, 1, true>));
+		k_q8_few<T, GATED, 1, true><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
+	}
+	else if(MR == 1) k_q8_few<T, GATED, 1, false><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
+	else if(MR == 2) k_q8_few<T, GATED, 2, false><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
+	else {
+		CLA_HIP(allow_full_lds((const void*) k_q8_few<T, GATED, 4, false>));
+		k_q8_few<T, GATED, 4, false><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
+	}
 	CLA_HIP(hipGetLastError());
 	return 0;
 }
@@ -280,7 +338,7 @@ template <class T, bool GATED>
 static int q8_mm(const Q8Product& p, hipStream_t stream) {
 	const int N = GATED ? p.N / 2 : p.N; // columns of the output
 	if(p.m <= Q8_FEW)
-		return q8_few<T, GATED>(Q8Few<T>{p.W, p.ldW, p.t, p.Q, p.ldQ, p.s, (int32_t) p.m, p.K, N, p.act, (const T*) p.bias, (T*) p.out, p.ldOut}, stream);
+		return q8_few<T, GATED>(Q8Few<T>{p.W, p.ldW, p.t, p.Q, p.ldQ, p.s, (int32_t) p.m, p.K, N, p.act, (const T*) p.bias, (T*) p.out, p.ldOut, (const T*) p.Y, p.ldY}, stream);
 	MmArgs A{};
 	A.rows = (const char*) p.Q; A.ldRows = p.ldQ;
 	A.cols = (const char*) p.W; A.ldCols = p.ldW;
@@ -292,6 +350,8 @@ static int q8_mm(const Q8Product& p, hipStream_t stream) {
 	if(mid >= g_numCU) return q8_tile<T, GATED, 128, 128>(A, epi, stream);
 	return q8_tile<T, GATED, 64, 128>(A, epi, stream);
 }
+
+bool q8_fuses(int64_t m, int64_t K) { return m <= Q8_FUSE && m * ((K + 15) & ~(int64_t) 15) <= Q8_FUSE_LDS; }
 
 int launch_q8(const Q8Product& p, int type, bool gated, hipStream_t stream) {
 	if(p.m == 0) return 0;

@@ -13,7 +13,11 @@ struct Q8Product {
 	int32_t K, N, act;
 	const void* bias;
 	void* out; int64_t ldOut;
+	const void* Y; int64_t ldY;                                 // rows as they come, in place of Q and s (q8_fuses); null otherwise
 };
+
+// Whether the product quantises so few and short rows itself.
+bool q8_fuses(int64_t m, int64_t K);
 
 int launch_q8_rows(const void* Y, int type, int64_t m, int K, int64_t ld, int8_t* Q, int64_t ldQ, float* scale, hipStream_t stream);
 int launch_q8_layout(const int8_t* src, int64_t ld, int byColumn, int64_t K, int N, int8_t* W, int64_t ldW, hipStream_t stream);
