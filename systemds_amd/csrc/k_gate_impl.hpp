@@ -73,7 +73,7 @@ static int gate_few(const GateFew<T>& A, hipStream_t stream) {
 
 template <class T, int TM, int TN, bool GATED, bool DIRECT, class Epi>
 static int gate_tile(MmArgs A, const Epi& epi, hipStream_t stream) {
-	constexpr int WM = 2, WN = 2, NF = TN / WN / MmOp<T>::FR;
+	constexpr int WM = 2, WN = TM == 256 ? 4 : 2, NF = TN / WN / MmOp<T>::FR;
 	constexpr size_t lds = std::max(2 * (TM + TN) * 128, WM * WN * Epi::template region<T, NF, GATED>());
 	A.tilesM = (int32_t) ((A.M + TM - 1) / TM);
 	A.tilesN = (A.N + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN);

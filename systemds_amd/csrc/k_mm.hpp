@@ -210,7 +210,7 @@ constexpr int64_t MM_MAX_LD = 4 << 20;   // bytes: a tile's offsets (256 rows) s
 // E: operands, TM x TN: rows and columns (gated: TN / 2 columns of either projection) of a tile, WM x WN waves. DIRECT: operands whose rows begin
 // and end at multiples of 16 bytes go from global memory to LDS without registers; others are loaded a step ahead into registers.
 template <class E, int TM, int TN, int WM, int WN, bool GATED, bool DIRECT, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, TM * TN / (WM * WN) >= 128 * 128 ? 1 : 2) void k_mm(MmArgs A, Epi epi) {
+__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >= 128 * 128 ? 1 : 2) void k_mm(MmArgs A, Epi epi) {
 #ifdef __HIP_DEVICE_COMPILE__ // (the host pass knows no buffer descriptors)
 	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
 	typedef MmOp<E> Op;

@@ -323,7 +323,7 @@ static int q8_few(const Q8Few<T>& A, hipStream_t stream) {
 
 template <class T, bool GATED, int TM, int TN>
 static int q8_tile(MmArgs A, const MmEpiOut<T, true>& epi, hipStream_t stream) {
-	constexpr int WM = 2, WN = 2, NF = TN / WN / 32;
+	constexpr int WM = 2, WN = TM == 256 ? 4 : 2, NF = TN / WN / 32;
 	constexpr size_t lds = std::max(2 * (TM + TN) * 128, WM * WN * MmEpiOut<T, true>::template region<int8_t, NF, GATED>());
 	A.tilesM = (int32_t) ((A.M + TM - 1) / TM);
 	A.tilesN = (A.N + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN);
