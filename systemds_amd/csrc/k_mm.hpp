@@ -254,19 +254,19 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 		if(GATED) rUp = __builtin_amdgcn_make_buffer_rsrc((void*) pUp, 0, colsIn * ldC, 0x00020000);
 	}
 	mm_i32x4 hold[DIRECT ? 1 : LM + LN];
-	auto issue = [&](int t) { // step t's operands: on their way to LDS (buffer t % 2), or into registers
+	auto issue = [&](int t, int which) { // step t's rows (1), columns (2): on their way to LDS (buffer t % 2), or into registers
 		const int k = t * 128;
 		if(DIRECT) {
 			char* const to = mm_smem + (t & 1) * BUF;
 			const bool out = k + piece >= K;
 			const unsigned vr = out ? MM_OUT : (unsigned) (lr * ldR + piece), vc = out ? MM_OUT : (unsigned) (lr * ldC + piece);
 #pragma unroll
-			for(int j = 0; j < LM; j++) {
+			for(int j = 0; j < (which & 1 ? LM : 0); j++) {
 				const int i = j * NW + wave;
 				__builtin_amdgcn_raw_ptr_buffer_load_lds(rRows, (__attribute__((address_space(3))) void*) (to + i * 1024), 16, (int) (vr + (unsigned) (i * 8 * ldR)), k, 0, 0);
 			}
 #pragma unroll
-			for(int j = 0; j < LN; j++) {
+			for(int j = 0; j < (which & 2 ? LN : 0); j++) {
 				const int i = j * NW + wave;
 				__builtin_amdgcn_raw_ptr_buffer_load_lds(col_half(i) ? rUp : rCols, (__attribute__((address_space(3))) void*) (to + TM * 128 + i * 1024), 16,
 					(int) (vc + (unsigned) (col_row(i) * ldC)), k, 0, 0);
@@ -317,10 +317,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 	};
 
 	if(nk > 0) {
-		issue(0);
+		issue(0, 3);
 		if(DIRECT) {
 			if(nk > 1) {
-				issue(1);
+				issue(1, 3);
 				asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LM + LN) : "memory");
 			}
 			else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -330,16 +330,18 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 		read(0, 0, 0);
 	}
 	for(int t = 0; t < nk; t++) {
-		if(!DIRECT && t + 1 < nk) issue(t + 1);
+		if(!DIRECT && t + 1 < nk) issue(t + 1, 3);
 #pragma unroll
 		for(int s = 0; s < SUB; s++) {
+			// (a step's columns follow its rows a part of a step later: a wave cannot issue anything else while its copies wait in line)
+			if(DIRECT && s == 0 && t > 0 && t + 1 < nk) issue(t + 1, 2);
 			if(s + 1 < SUB) read((s + 1) & 1, t, s + 1);
 			else if(t + 1 < nk) {
 				// everything of step t has been read; step t + 1 was requested a step ago
 				if(DIRECT) {
 					asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 					barrier();
-					if(t + 2 < nk) issue(t + 2);
+					if(t + 2 < nk) issue(t + 2, 1);
 				}
 				else {
 					put(t + 1); // (its buffer was last read in step t - 1)
@@ -351,6 +353,14 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 			for(int i = 0; i < NF; i++)
 #pragma unroll
 				for(int j = 0; j < MF; j++) Op::mma(acc[i][j], fc[s & 1][i], fr[s & 1][j]);
+			if(sizeof(E) <= 2) { // the next reads and copies between the products, not in front of them
+#pragma unroll
+				for(int q = 0; q < NF * MF; q++) {
+					__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                   // a product
+					if(q < NF + MF) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);   // an LDS read
+					if(q < LM) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);        // a copy
+				}
+			}
 		}
 	}
 	barrier(); // LDS is the epilogue's
