@@ -6,25 +6,35 @@
 
 namespace cla {
 
+// Parts of a sum of `steps` steps of 128 bytes: two tiles for every CU where there are not enough, at least 8 steps each.
+static int64_t gate_parts(int64_t rows, int64_t cols, int64_t steps) {
+	const int64_t tiles = ((rows + 127) / 128) * ((cols + 127) / 128);
+	if(tiles >= g_numCU) return 1;
+	return std::max<int64_t>(1, std::min((2 * g_numCU + tiles - 1) / tiles, steps / 8));
+}
+
 GatePlan gate_plan(int type, int64_t m, int nIn, int nOut) {
 	GatePlan p{};
 	const int64_t es = (int64_t) type_bytes(type), calc = type == CLA_F64 ? 8 : 4, F = nOut;
 	p.half = (int64_t) up((size_t) F, (size_t) (16 / es));
-	// the weights' gradient: parts of the batch until there are two tiles for every CU, at least 512 rows each
-	const int64_t tiles = ((2 * F + 127) / 128) * (((int64_t) nIn + 127) / 128);
-	const int64_t want = tiles >= g_numCU ? 1 : (2 * g_numCU + tiles - 1) / tiles;
-	const int64_t parts = std::max<int64_t>(1, std::min(want, m / 512));
+	const int64_t stepsY = (2 * p.half * es + 127) / 128, partsY = gate_parts(m, nIn, stepsY);
+	p.kPartY = (stepsY + partsY - 1) / partsY * 128;
+	p.partsY = (int32_t) ((stepsY * 128 + p.kPartY - 1) / p.kPartY);
+	const int64_t parts = gate_parts(2 * F, nIn, m * es / 128);
 	p.kPart = std::min((int64_t) up((size_t) ((std::max<int64_t>(m, 1) + parts - 1) / parts), 256), ((int64_t) 4 << 20) / es);
 	p.parts = (int32_t) std::max<int64_t>(1, (m + p.kPart - 1) / p.kPart);
 	p.sumRows = (int32_t) ((m + 31) / 32);
+	p.sumJoins = (p.sumRows + 63) / 64;
 	size_t at = 0;
 	auto take = [&](int64_t bytes) { const size_t from = at; at += up((size_t) bytes, 256); return from; };
 	p.P = take(m * 2 * p.half * es);
 	p.Pt = take((int64_t) p.parts * 2 * F * p.kPart * es);
 	p.Wt = take(nIn * 2 * p.half * es);
 	p.Yt = take((int64_t) p.parts * nIn * p.kPart * es);
+	p.joinsY = take(p.partsY > 1 ? (int64_t) p.partsY * m * nIn * calc : 0);
 	p.joins = take(p.parts > 1 ? (int64_t) p.parts * 2 * F * nIn * calc : 0);
 	p.sums = take((int64_t) p.sumRows * 2 * F * calc);
+	p.sums64 = take((int64_t) p.sumJoins * 2 * F * calc);
 	p.bytes = at;
 	return p;
 }

@@ -18,12 +18,13 @@ struct GateCall {
 	char* ws;
 };
 
-// The backward pass's workspace: bytes from its start.
+// The backward pass's parts and workspace (bytes from its start).
 struct GatePlan {
 	int64_t half;                       // columns of a half of P, rounded up to 16 bytes
-	int64_t kPart; int32_t parts;       // rows of the batch summed at a time for dW
-	int32_t sumRows;                    // partial sums for dB: at most so many rows
-	size_t P, Pt, Wt, Yt, joins, sums, bytes;
+	int64_t kPartY; int32_t partsY;     // dY: bytes of the columns of P summed at a time (a multiple of 128)
+	int64_t kPart; int32_t parts;       // dW: rows of the batch summed at a time (a multiple of 256)
+	int32_t sumRows, sumJoins;          // dB: partial sums of a wave's rows (at most so many), and of 64 of those
+	size_t P, Pt, Wt, Yt, joinsY, joins, sums, sums64, bytes;
 };
 
 GatePlan gate_plan(int type, int64_t m, int nIn, int nOut);

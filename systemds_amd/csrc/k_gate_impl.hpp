@@ -2,8 +2,9 @@
 //
 // Forward: one kernel; a tile holds as many columns of either projection, a wave both values of an output, so the activation and the product are its
 // epilogue. 16-bit operands are summed in fp32, fp32 in fp32, fp64 in fp64.
-// Backward: the projections again (cheaper than 2 nRowY x nOut values kept by every layer between the passes), with dG and dU as the epilogue, then
-//   dY = [dG dU] [Wg; Wu],   dW = t([dG dU]) Y,   db = column sums of [dG dU].
+// Backward, three or four launches: the projections again (cheaper than 2 nRowY x nOut values kept by every layer between the passes), with dG and dU as the epilogue; then
+//   dY = [dG dU] [Wg; Wu],   dW = t([dG dU]) Y,   db = column sums of [dG dU]
+// together; then the sums that were split.
 // The tiles want both operands by rows of the summed index, so dG and dU are written by row and by column, W and Y are transposed into the workspace. dG and dU are
 // rounded to T between the products: the matrix cores take no wider operand, and a rounding of 2^-9 (bf16) of each of many terms leaves less than the result's own.
 // Sums over the batch for few weights are split into parts, joined in their order: results do not depend on timing.
@@ -32,7 +33,9 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_gate_few(GateFew<T> A) {
 	extern __shared__ __attribute__((aligned(16))) char gate_smem[]; // [wave][half][row][column]
 	typedef typename MmCalc<T>::type C;
 	typedef typename MmOp<T>::Acc16 Acc;
-	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MR;
+	A.Y += m0 * A.ldY; A.out += m0 * A.ld;
+	A.m = min(A.m - m0, 16 * MR);
 	Acc acc[2][MR];
 	auto rowOf = [&](int row, int64_t k, int64_t left) { return mm_load16<sizeof(T)>((const char*) (A.Y + (row < A.m ? row : 0) * A.ldY) + k, row < A.m ? left : 0); };
 	mm_few<T, true, MR>((const char*) A.W, A.ldW * (int64_t) sizeof(T), n0, A.nOut, (int64_t) A.nIn * sizeof(T), rowOf, [] {}, acc, wave, lane);
@@ -61,27 +64,12 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_gate_few(GateFew<T> A) {
 
 template <class T>
 static int gate_few(const GateFew<T>& A, hipStream_t stream) {
-	const unsigned grid = (unsigned) ((A.nOut + 15) / 16);
-	const int MR = A.m <= 16 ? 1 : A.m <= 32 ? 2 : 4;
+	const int MR = std::min(mm_few_rows(A.m, A.nOut, g_numCU), sizeof(T) == 8 ? 2 : 4); // (64 rows of fp64 do not fit the registers)
+	const dim3 grid((unsigned) ((A.nOut + 15) / 16), (unsigned) ((A.m + 16 * MR - 1) / (16 * MR)));
 	const size_t lds = (size_t) MMF_WAVES * 2 * MR * 256 * sizeof(typename MmCalc<T>::type);
-	auto kernel = MR == 1 ? k_gate_few<T, 1> : MR == 2 ? k_gate_few<T, 2> : k_gate_few<T, 4>;
+	auto kernel = MR == 1 ? k_gate_few<T, 1> : MR == 2 ? k_gate_few<T, 2> : k_gate_few<T, sizeof(T) == 8 ? 2 : 4>;
 	if(lds > 65536) CLA_HIP(allow_full_lds((const void*) kernel));
 	kernel<<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
-	CLA_HIP(hipGetLastError());
-	return 0;
-}
-
-template <class T, int TM, int TN, bool GATED, bool DIRECT, class Epi>
-static int gate_tile(MmArgs A, const Epi& epi, hipStream_t stream) {
-	constexpr int WM = 2, WN = TM == 256 ? 4 : 2, NF = TN / WN / MmOp<T>::FR;
-	constexpr size_t lds = std::max(2 * (TM + TN) * 128, WM * WN * Epi::template region<T, NF, GATED>());
-	A.tilesM = (int32_t) ((A.M + TM - 1) / TM);
-	A.tilesN = (A.N + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN);
-	const int64_t grid = (int64_t) A.tilesM * A.tilesN * A.parts;
-	if(grid > 0x7fffffffLL) { set_error("gate: a product of %lld tiles", (long long) grid); return -CLA_ERR_UNSUPPORTED; }
-	auto kernel = k_mm<T, TM, TN, WM, WN, GATED, DIRECT, Epi>;
-	CLA_HIP(allow_full_lds((const void*) kernel));
-	kernel<<<(unsigned) grid, 64 * WM * WN, lds, stream>>>(A, epi);
 	CLA_HIP(hipGetLastError());
 	return 0;
 }
@@ -92,29 +80,78 @@ static inline bool gate_direct(const MmArgs& A) {
 		A.ldCols <= MM_MAX_LD;
 }
 
-// Rows of a tile: the largest tile of which there are enough for the chip.
+// A tile's shape (TM * 1000 + TN; 64129: 64 x 128 with four steps in LDS, which takes a CU for itself). 16-bit types: the largest of which there is one for every CU
+// (fewer, larger tiles read less through LDS, which is what small ones are bound by). fp32 and fp64 are bound by their matrix instructions at any size: the shape whose tiles leave the busiest CU the least.
 template <class T>
-static int gate_tile_rows(const MmArgs& A, bool gated) {
+static int gate_shape(const MmArgs& A, bool gated) {
 	const int64_t n = gated ? 2 * (int64_t) A.N : A.N;
 	auto tiles = [&](int tm, int tn) { return ((A.M + tm - 1) / tm) * ((n + tn - 1) / tn) * A.parts; };
-	if(sizeof(T) == 2 && gate_direct(A) && tiles(256, 256) >= g_numCU) return 256;
-	return tiles(128, 128) >= g_numCU ? 128 : 64;
+	if(sizeof(T) == 2) {
+		if(gate_direct(A) && tiles(256, 256) >= g_numCU) return 256256;
+		if(tiles(128, 128) >= g_numCU) return 128128;
+		return gate_direct(A) && tiles(64, 128) <= g_numCU ? 64129 : 64128;
+	}
+	int best = 0;
+	int64_t least = 0;
+	for(const int shape : {128128, 64128, 64064}) {
+		const int tm = shape / 1000, tn = shape % 1000;
+		const int64_t cost = (tiles(tm, tn) + g_numCU - 1) / g_numCU * tm * tn;
+		if(best == 0 || cost < least) { best = shape; least = cost; }
+	}
+	return best;
 }
 
-template <class T, bool GATED, class Epi>
-static int gate_mm(const MmArgs& A, const Epi& epi, hipStream_t stream) {
-	const int rows = gate_tile_rows<T>(A, GATED);
-	if(gate_direct(A)) {
-		if constexpr(sizeof(T) == 2) {
-			if(rows == 256) return gate_tile<T, 256, 256, GATED, true>(A, epi, stream);
-		}
-		return rows == 128 ? gate_tile<T, 128, 128, GATED, true>(A, epi, stream) : gate_tile<T, 64, 128, GATED, true>(A, epi, stream);
-	}
-	if constexpr(GATED) // (the other products read what this file has laid out)
-		return rows == 128 ? gate_tile<T, 128, 128, GATED, false>(A, epi, stream) : gate_tile<T, 64, 128, GATED, false>(A, epi, stream);
-	set_error("gate: operands of a product in the workspace are not aligned");
-	return -CLA_ERR_STATE;
+template <class Shape>
+static int64_t gate_tiles(MmArgs& A) {
+	constexpr int cols = Shape::GATED ? Shape::TN / 2 : Shape::TN;
+	A.tilesM = (int32_t) ((A.M + Shape::TM - 1) / Shape::TM);
+	A.tilesN = (A.N + cols - 1) / cols;
+	return (int64_t) A.tilesM * A.tilesN * A.parts;
 }
+
+static inline int gate_grid(int64_t blocks) {
+	if(blocks <= 0x7fffffffLL) return 0;
+	set_error("gate: a product of %lld tiles", (long long) blocks);
+	return -CLA_ERR_UNSUPPORTED;
+}
+
+// Calls launch(Shape()) with the shape of that number.
+template <class T, bool GATED, bool DIRECT, class Launch>
+static int gate_with(int shape, const Launch& launch) {
+	if constexpr(sizeof(T) == 2) {
+		if constexpr(DIRECT) {
+			if(shape == 256256) return launch(MmShape<T, 256, 256, 2, 4, 2, GATED, DIRECT>());
+			if(shape == 64129) return launch(MmShape<T, 64, 128, 2, 2, 4, GATED, DIRECT>());
+		}
+	}
+	else {
+		if(shape == 64064) return launch(MmShape<T, 64, 64, 2, 2, 2, GATED, DIRECT>());
+	}
+	if(shape == 128128) return launch(MmShape<T, 128, 128, 2, 2, 2, GATED, DIRECT>());
+	return launch(MmShape<T, 64, 128, 2, 2, 2, GATED, DIRECT>());
+}
+
+// The projections of a gated unit, with more blocks of other work behind them.
+template <class T, class Epi, class More>
+static int gate_project(MmArgs A, const Epi& epi, int64_t moreBlocks, const More& more, hipStream_t stream) {
+	const int shape = gate_shape<T>(A, true);
+	auto launch = [&](auto s) {
+		typedef decltype(s) Shape;
+		const int64_t blocks = gate_tiles<Shape>(A);
+		if(const int rc = gate_grid(blocks + moreBlocks)) return rc;
+		auto kernel = k_mm_and<Shape, Epi, More>;
+		CLA_HIP(allow_full_lds((const void*) kernel));
+		kernel<<<(unsigned) (blocks + moreBlocks), Shape::THREADS, std::max(Shape::template lds<Epi>(), More::LDS), stream>>>(A, epi, (unsigned) blocks, more);
+		CLA_HIP(hipGetLastError());
+		return 0;
+	};
+	return gate_direct(A) ? gate_with<T, true, true>(shape, launch) : gate_with<T, true, false>(shape, launch);
+}
+
+struct GateNothing {
+	static constexpr size_t LDS = 0;
+	__device__ void run(unsigned, char*) const {}
+};
 
 template <class T>
 static MmArgs gate_args(const GateCall& c) {
@@ -128,59 +165,130 @@ static MmArgs gate_args(const GateCall& c) {
 template <class T>
 static bool whole(const void* p, int64_t ld) { return (((uintptr_t) p | (uintptr_t) (ld * (int64_t) sizeof(T))) & 15) == 0; }
 
-constexpr int GATE_FEW = 64;
-
 template <class T>
 int gate_forward(const GateCall& c, hipStream_t stream) {
-	if(c.m <= GATE_FEW)
+	if(mm_few_suits<T>(c.m, c.nOut, g_numCU))
 		return gate_few<T>(GateFew<T>{(const T*) c.Y, c.ldY, (const T*) c.W, c.ldW, (int32_t) c.m, c.nIn, c.nOut, c.act, (const T*) c.bias, (T*) c.out, c.ldOut}, stream);
 	const MmEpiOut<T, false> epi{nullptr, nullptr, (const T*) c.bias, (T*) c.out, c.ldOut, c.act, whole<T>(c.out, c.ldOut), 0};
-	return gate_mm<T, true>(gate_args<T>(c), epi, stream);
+	return gate_project<T>(gate_args<T>(c), epi, 0, GateNothing(), stream);
 }
 
-// dst[part][c][r] = src[part * kPart + r][c] for rows r < R, zeros behind them up to padR. Bound: the bytes once in, once out.
-template <class U>
-__global__ __launch_bounds__(256) void k_mm_transpose(const U* __restrict__ src, int64_t ld, int64_t R, int Cn, U* __restrict__ dst, int64_t ldDst, int64_t zDst,
-	int64_t padR, int64_t kPart) {
-	__shared__ U tile[64][64 + 4 / sizeof(U) + 1];
-	const int64_t r0 = (int64_t) blockIdx.x * 64;
-	const int c0 = blockIdx.y * 64;
-	const int a = threadIdx.x & 63, b = threadIdx.x >> 6;
-	for(int i = b; i < 64; i += 4) tile[i][a] = r0 + i < R && c0 + a < Cn ? src[(r0 + i) * ld + c0 + a] : (U) 0;
-	__syncthreads();
-	const int64_t part = r0 / kPart, at = r0 - part * kPart;
-	if(r0 + a < padR)
-		for(int i = b; i < 64; i += 4)
-			if(c0 + i < Cn) dst[part * zDst + (int64_t) (c0 + i) * ldDst + at + a] = tile[a][i];
-}
-
-// out = the sum of the parts, in their order
-template <class T>
-__global__ __launch_bounds__(256) void k_mm_join(const typename MmCalc<T>::type* __restrict__ part, int parts, int64_t rows, int cols, T* __restrict__ out, int64_t ld) {
-	typedef typename MmCalc<T>::type C;
-	const int64_t n = rows * cols;
-	for(int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
-		C s = C(0);
-		for(int p = 0; p < parts; p++) s += part[p * n + i];
-		out[i / cols * ld + i % cols] = (T) s;
+// dst[part][c][r] = src[part * kPart + r][c] for rows r < R, zeros behind them up to padR; a block takes 64 x 64 of it.
+struct GateTranspose {
+	const void* src; int64_t ld, R; int32_t cols;
+	void* dst; int64_t ldDst, zDst, padR, kPart;
+	unsigned blocksR, blocks;   // 0 blocks: nothing to do
+	static GateTranspose of(const void* src, int64_t ld, int64_t R, int cols, void* dst, int64_t ldDst, int64_t zDst, int64_t padR, int64_t kPart) {
+		const int64_t r = (padR + 63) / 64;
+		return {src, ld, R, cols, dst, ldDst, zDst, padR, kPart, (unsigned) r, (unsigned) (r * ((cols + 63) / 64))};
 	}
+};
+
+// The backward pass's other layouts: both halves of t(W) and t(Y). Bound: the bytes once in, once out, 16 of them a lane.
+template <class U> struct GateLayouts {
+	GateTranspose t[3];
+	static constexpr int PITCH = 64 + (sizeof(U) == 2 ? 2 : 1);
+	static constexpr size_t LDS = 64 * PITCH * sizeof(U);
+	__device__ __forceinline__ void run(unsigned block, char* smem) const {
+		constexpr int V = 16 / (int) sizeof(U), PER = 64 / V;
+		U* const tile = (U*) smem;
+		const int i = block < t[0].blocks ? 0 : block - t[0].blocks < t[1].blocks ? 1 : 2;
+		if(i > 0) block -= t[0].blocks;
+		if(i > 1) block -= t[1].blocks;
+		const GateTranspose g = t[i];
+		const U* const src = (const U*) g.src;
+		U* const dst = (U*) g.dst;
+		const int64_t r0 = (int64_t) (block % g.blocksR) * 64;
+		const int c0 = (int) (block / g.blocksR) * 64, a = threadIdx.x % PER * V, step = blockDim.x / PER;
+		const bool aligned = (((uintptr_t) src | (uintptr_t) (g.ld * sizeof(U))) & 15) == 0;
+		for(int b = threadIdx.x / PER; b < 64; b += step) {
+			MmPack<U, V> p;
+			const bool in = r0 + b < g.R;
+			const U* const from = src + (r0 + b) * g.ld + c0 + a;
+			if(in && aligned && c0 + a + V <= g.cols) p = *(const MmPack<U, V>*) from;
+			else {
+#pragma unroll
+				for(int v = 0; v < V; v++) p.x[v] = in && c0 + a + v < g.cols ? from[v] : (U) 0;
+			}
+#pragma unroll
+			for(int v = 0; v < V; v++) tile[b * PITCH + a + v] = p.x[v];
+		}
+		__syncthreads();
+		const int64_t part = r0 / g.kPart, at = r0 - part * g.kPart;
+		for(int b = threadIdx.x / PER; b < 64; b += step) { // (padR and the rows' starts are multiples of 16 bytes)
+			if(c0 + b >= g.cols || r0 + a >= g.padR) continue;
+			MmPack<U, V> p;
+#pragma unroll
+			for(int v = 0; v < V; v++) p.x[v] = tile[(a + v) * PITCH + b];
+			*(MmPack<U, V>*) (dst + part * g.zDst + (int64_t) (c0 + b) * g.ldDst + at + a) = p;
+		}
+	}
+};
+
+template <class U>
+__global__ __launch_bounds__(256) void k_gate_layouts(GateLayouts<U> lay) {
+	__shared__ __attribute__((aligned(16))) char smem[GateLayouts<U>::LDS];
+	lay.run(blockIdx.x, smem);
 }
 
-// Column sums of rows of partial sums: 64 columns a block, its 16 waves every 16th row, joined in the order of the waves.
+// Sums of 64 rows of partial sums at a time: a block takes 64 columns of them, its waves 64 rows each.
+template <class C> struct GateSums {
+	const C* part; C* out;
+	int32_t rows, cols, groups;
+	unsigned blocksC;
+	static constexpr size_t LDS = 0;
+	__device__ __forceinline__ void run(unsigned block, char*) const {
+		const int col = (int) (block % blocksC) * 64 + (threadIdx.x & 63), group = (int) (block / blocksC) * (blockDim.x / 64) + (threadIdx.x >> 6);
+		if(col >= cols || group >= groups) return;
+		const int r0 = group * 64, n = min(64, rows - r0);
+		const C* const p = part + (int64_t) r0 * cols + col;
+		C s = C(0);
+#pragma unroll 8
+		for(int r = 0; r < n; r++) s += p[(int64_t) r * cols];
+		out[(int64_t) group * cols + col] = s;
+	}
+};
+
+// out = the sum of the parts: a block takes 64 values, each of its waves a quarter of the parts, in their order.
+template <class T> struct GateJoin {
+	const typename MmCalc<T>::type* part;
+	T* out;
+	int64_t rows, ld;
+	int32_t cols, parts;
+	unsigned blocks;            // 0: nothing to do
+	static GateJoin of(const typename MmCalc<T>::type* part, T* out, int64_t rows, int cols, int64_t ld, int parts) {
+		return {part, out, rows, ld, cols, parts, (unsigned) std::min<int64_t>((rows * cols + 63) / 64, 1 << 20)};
+	}
+};
+
+template <class T> struct GateJoins { GateJoin<T> j[3]; };
+
 template <class T>
-__global__ __launch_bounds__(1024) void k_gate_sums(const typename MmCalc<T>::type* __restrict__ part, int rows, int cols, T* __restrict__ out) {
+__global__ __launch_bounds__(256) void k_gate_join(GateJoins<T> all) {
 	typedef typename MmCalc<T>::type C;
-	__shared__ C red[16][64];
-	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = blockIdx.x * 64 + lane;
-	C s = C(0);
-	if(col < cols)
-		for(int r = wave; r < rows; r += 16) s += part[(int64_t) r * cols + col];
-	red[wave][lane] = s;
-	__syncthreads();
-	if(wave == 0 && col < cols) {
+	__shared__ C red[4][64];
+	unsigned block = blockIdx.x;
+	const int i = block < all.j[0].blocks ? 0 : block - all.j[0].blocks < all.j[1].blocks ? 1 : 2;
+	if(i > 0) block -= all.j[0].blocks;
+	if(i > 1) block -= all.j[1].blocks;
+	const GateJoin<T> g = all.j[i];
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (g.parts + 3) / 4, p0 = min(wave * per, g.parts), p1 = min(p0 + per, g.parts);
+	const int64_t n = g.rows * g.cols;
+	for(int64_t v0 = (int64_t) block * 64; v0 < n; v0 += (int64_t) g.blocks * 64) {
+		const int64_t v = v0 + lane;
+		C s = C(0);
+		if(v < n) {
+#pragma unroll 4
+			for(int p = p0; p < p1; p++) s += g.part[p * n + v];
+		}
+		red[wave][lane] = s;
+		__syncthreads();
+		if(wave == 0 && v < n) {
 #pragma unroll
-		for(int w = 1; w < 16; w++) s += red[w][lane];
-		out[col] = (T) s;
+			for(int w = 1; w < 4; w++) s += red[w][lane];
+			g.out[v / g.cols * g.ld + v % g.cols] = (T) s;
+		}
+		__syncthreads();
 	}
 }
 
@@ -195,13 +303,23 @@ template <> struct MmBits<float> { typedef uint32_t type; };
 template <> struct MmBits<__bf16> { typedef uint16_t type; };
 template <> struct MmBits<_Float16> { typedef uint16_t type; };
 
-template <class T>
-static int gate_transpose(const void* src, int64_t ld, int64_t R, int Cn, void* dst, int64_t ldDst, int64_t zDst, int64_t padR, int64_t kPart, hipStream_t stream) {
-	typedef typename MmBits<T>::type U;
-	k_mm_transpose<U><<<dim3((unsigned) ((padR + 63) / 64), (unsigned) ((Cn + 63) / 64)), 256, 0, stream>>>((const U*) src, ld, R, Cn, (U*) dst, ldDst, zDst, padR, kPart);
-	CLA_HIP(hipGetLastError());
-	return 0;
-}
+// Where a product goes: T, or (parts > 1) partial sums. One type for both, so that one kernel holds either product.
+template <class T> struct GateOut {
+	MmEpiOut<T, false> whole;
+	MmEpiOut<typename MmCalc<T>::type, false> part;
+	int32_t parts;
+	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
+	template <class E, int MF, int NF, bool GATED, class Acc>
+	__device__ __forceinline__ void run(Acc& acc, char* region, int64_t m0, int n0, int64_t M, int N, int p, int rowPart, int lane) const {
+		if(parts == 1) whole.template run<E, MF, NF, GATED>(acc, region, m0, n0, M, N, p, rowPart, lane);
+		else part.template run<E, MF, NF, GATED>(acc, region, m0, n0, M, N, p, rowPart, lane);
+	}
+	static GateOut of(T* out, int64_t ld, typename MmCalc<T>::type* joins, int64_t M, int64_t N, int parts) {
+		typedef typename MmCalc<T>::type C;
+		return {{nullptr, nullptr, nullptr, out, ld, ACT_NONE, ::cla::whole<T>(out, ld), 0},
+			{nullptr, nullptr, nullptr, joins, N, ACT_NONE, ::cla::whole<C>(joins, N), M * N}, parts};
+	}
+};
 
 template <class T>
 int gate_backward(const GateCall& c, hipStream_t stream) {
@@ -215,48 +333,71 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 		CLA_HIP(hipGetLastError());
 		return 0;
 	}
+	typedef typename MmBits<T>::type U;
 	const GatePlan p = gate_plan(c.type, c.m, c.nIn, c.nOut);
 	T* const P = (T*) (c.ws + p.P);
 	T* const Pt = (T*) (c.ws + p.Pt);
 	T* const Wt = (T*) (c.ws + p.Wt);
 	T* const Yt = (T*) (c.ws + p.Yt);
 	C* const sums = (C*) (c.ws + p.sums);
+	C* const sums64 = (C*) (c.ws + p.sums64);
+	const int64_t pad = (c.m + V - 1) / V * V;
+
+	// projections, dG and dU; W and Y the other way round
+	const MmArgs project = gate_args<T>(c);
 	const MmEpiBack<T> back{(const T*) c.bias, (const T*) c.D, c.ldD, c.dY ? P : nullptr, 2 * p.half, c.dW ? Pt : nullptr, p.kPart, c.dB ? sums : nullptr, c.act,
 		whole<T>(c.D, c.ldD)};
-	const MmArgs again = gate_args<T>(c);
-	if((rc = gate_mm<T, true>(again, back, stream))) return rc;
-	if(c.dB) {
-		const int waveRows = gate_tile_rows<T>(again, true) / 2, rows = (int) ((c.m + waveRows - 1) / waveRows); // (a row of partial sums per wave)
-		k_gate_sums<T><<<(unsigned) ((2 * F + 63) / 64), 1024, 0, stream>>>(sums, rows, (int) (2 * F), (T*) c.dB);
-		CLA_HIP(hipGetLastError());
-	}
-	if(c.dY) {
+	GateLayouts<U> lay{};
+	const int64_t one = (int64_t) 1 << 40; // (a single part)
+	if(c.dY)
 		for(int h = 0; h < 2; h++)
-			if((rc = gate_transpose<T>((const T*) c.W + h * F * c.ldW, c.ldW, F, c.nIn, Wt + h * p.half, 2 * p.half, 0, p.half, (int64_t) 1 << 40, stream))) return rc;
-		MmArgs A{};
-		A.rows = (const char*) P; A.ldRows = 2 * p.half * es;
-		A.cols = (const char*) Wt; A.ldCols = 2 * p.half * es;
-		A.M = c.m; A.N = c.nIn; A.K = A.kPart = 2 * p.half * es; A.parts = 1;
-		const MmEpiOut<T, false> epi{nullptr, nullptr, nullptr, (T*) c.dY, c.ldDY, ACT_NONE, whole<T>(c.dY, c.ldDY), 0};
-		if((rc = gate_mm<T, false>(A, epi, stream))) return rc;
+			lay.t[h] = GateTranspose::of((const T*) c.W + h * F * c.ldW, c.ldW, F, c.nIn, Wt + h * p.half, 2 * p.half, 0, p.half, one);
+	if(c.dW) lay.t[2] = GateTranspose::of(c.Y, c.ldY, c.m, c.nIn, Yt, p.kPart, c.nIn * p.kPart, pad, p.kPart);
+	// few of them behind the projections' tiles, in the same launch; many in one of their own: a tile's LDS leaves a CU to one block (4096 x 4096 into 2 x 8192 on
+	// bf16 1.85 ms in all, 1.49 so)
+	int64_t lays = (int64_t) lay.t[0].blocks + lay.t[1].blocks + lay.t[2].blocks;
+	if(lays > 2 * g_numCU) {
+		if((rc = gate_grid(lays))) return rc;
+		k_gate_layouts<U><<<(unsigned) lays, 256, 0, stream>>>(lay);
+		lays = 0;
 	}
-	if(c.dW) {
-		const int64_t pad = (c.m + V - 1) / V * V;
-		if((rc = gate_transpose<T>(c.Y, c.ldY, c.m, c.nIn, Yt, p.kPart, c.nIn * p.kPart, pad, p.kPart, stream))) return rc;
-		MmArgs A{};
-		A.rows = (const char*) Pt; A.ldRows = p.kPart * es; A.zRows = 2 * F * p.kPart * es;
-		A.cols = (const char*) Yt; A.ldCols = p.kPart * es; A.zCols = c.nIn * p.kPart * es;
-		A.M = 2 * F; A.N = c.nIn; A.K = pad * es; A.kPart = p.kPart * es; A.parts = p.parts;
-		if(p.parts == 1) {
-			const MmEpiOut<T, false> epi{nullptr, nullptr, nullptr, (T*) c.dW, c.ldDW, ACT_NONE, whole<T>(c.dW, c.ldDW), 0};
-			return gate_mm<T, false>(A, epi, stream);
-		}
-		C* const joins = (C*) (c.ws + p.joins);
-		const MmEpiOut<C, false> epi{nullptr, nullptr, nullptr, joins, c.nIn, ACT_NONE, whole<C>(joins, c.nIn), 2 * F * c.nIn};
-		if((rc = gate_mm<T, false>(A, epi, stream))) return rc;
-		k_mm_join<T><<<(unsigned) std::min<int64_t>((2 * F * c.nIn + 255) / 256, g_numCU * 8), 256, 0, stream>>>(joins, p.parts, 2 * F, c.nIn, (T*) c.dW, c.ldDW);
+	if((rc = gate_project<T>(project, back, lays, lay, stream))) return rc;
+
+	// dY = P W and dW = t(P) Y; the first sums of dB
+	MmArgs A{}, B{};
+	A.rows = (const char*) P; A.cols = (const char*) Wt; A.ldRows = A.ldCols = A.K = 2 * p.half * es;
+	A.M = c.dY ? c.m : 0; A.N = c.nIn; A.zRows = A.zCols = A.kPart = p.kPartY; A.parts = p.partsY;
+	B.rows = (const char*) Pt; B.cols = (const char*) Yt; B.ldRows = B.ldCols = B.kPart = p.kPart * es; B.K = pad * es;
+	B.zRows = 2 * F * p.kPart * es; B.zCols = c.nIn * p.kPart * es;
+	B.M = c.dW ? 2 * F : 0; B.N = c.nIn; B.parts = p.parts;
+	C* const joinsY = (C*) (c.ws + p.joinsY);
+	C* const joinsW = (C*) (c.ws + p.joins);
+	const GateOut<T> outY = GateOut<T>::of((T*) c.dY, c.ldDY, joinsY, c.m, c.nIn, p.partsY), outW = GateOut<T>::of((T*) c.dW, c.ldDW, joinsW, 2 * F, c.nIn, p.parts);
+	const int waveRows = gate_shape<T>(project, true) / 1000 / 2, sumRows = (int) ((c.m + waveRows - 1) / waveRows); // (a row of partial sums per wave)
+	GateSums<C> first{sums, sums64, sumRows, (int32_t) (2 * F), (sumRows + 63) / 64, (unsigned) ((2 * F + 63) / 64)};
+	MmArgs both = A; // (the shape that suits both: as many tiles as they have together)
+	both.M = A.M * A.parts + B.M * B.parts; both.parts = 1;
+	auto launch = [&](auto s) {
+		typedef decltype(s) Shape;
+		constexpr int waves = Shape::THREADS / 64;
+		const int64_t nA = gate_tiles<Shape>(A), nB = gate_tiles<Shape>(B), nC = c.dB ? (int64_t) first.blocksC * ((first.groups + waves - 1) / waves) : 0;
+		if(nA + nB + nC == 0) return 0;
+		if(const int r = gate_grid(nA + nB + nC)) return r;
+		auto kernel = k_mm_two<Shape, GateOut<T>, GateOut<T>, GateSums<C>>;
+		CLA_HIP(allow_full_lds((const void*) kernel));
+		kernel<<<(unsigned) (nA + nB + nC), Shape::THREADS, Shape::template lds<GateOut<T>>(), stream>>>(A, outY, (unsigned) nA, B, outW, (unsigned) nB, first);
 		CLA_HIP(hipGetLastError());
-	}
+		return 0;
+	};
+	if((rc = gate_with<T, false, true>(gate_shape<T>(both, false), launch))) return rc;
+
+	GateJoins<T> joins{};
+	if(c.dY && p.partsY > 1) joins.j[0] = GateJoin<T>::of(joinsY, (T*) c.dY, c.m, c.nIn, c.ldDY, p.partsY);
+	if(c.dW && p.parts > 1) joins.j[1] = GateJoin<T>::of(joinsW, (T*) c.dW, 2 * F, c.nIn, c.ldDW, p.parts);
+	if(c.dB) joins.j[2] = GateJoin<T>::of(sums64, (T*) c.dB, 1, (int) (2 * F), 2 * F, first.groups);
+	const unsigned blocks = joins.j[0].blocks + joins.j[1].blocks + joins.j[2].blocks;
+	if(blocks > 0) k_gate_join<T><<<blocks, 256, 0, stream>>>(joins);
+	CLA_HIP(hipGetLastError());
 	return 0;
 }
 

@@ -62,21 +62,17 @@ template <> struct MmOp<_Float16> {
 		c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(mm_f16x8, a), __builtin_bit_cast(mm_f16x8, b), c, 0, 0, 0);
 	}
 };
-template <> struct MmOp<float> {
-	static constexpr int FR = 32;
+template <> struct MmOp<float> { // (16 rows: the same rate, and tiles half as large)
+	static constexpr int FR = 16;
 	typedef float Sum;
-	typedef mm_f32x16 Acc;
+	typedef mm_f32x4 Acc;
 	typedef mm_f32x4 Acc16;
 	static __device__ __forceinline__ void mma(Acc& c, mm_i32x4 a, mm_i32x4 b) {
 		const mm_f32x4 x = __builtin_bit_cast(mm_f32x4, a), y = __builtin_bit_cast(mm_f32x4, b);
 #pragma unroll
-		for(int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i], y[i], c, 0, 0, 0);
-	}
-	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) {
-		const mm_f32x4 x = __builtin_bit_cast(mm_f32x4, a), y = __builtin_bit_cast(mm_f32x4, b);
-#pragma unroll
 		for(int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
 	}
+	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) { mma(c, a, b); }
 };
 template <> struct MmOp<double> {
 	static constexpr int FR = 16;
@@ -91,17 +87,12 @@ template <> struct MmOp<double> {
 	static __device__ __forceinline__ void mma16(Acc16& c, mm_i32x4 a, mm_i32x4 b) { mma(c, a, b); }
 };
 
-// The column (of a fragment) that result r of this lane belongs to; its row is lane % FR. Results come in groups of neighbouring columns
-// (four, or one of fp64).
+// The column (of a fragment) that result r of this lane belongs to; its row is lane % FR. Results come in groups of MmGroup neighbouring columns.
 template <class E>
-__device__ __forceinline__ int mm_col(int lane, int r) {
-	if(MmOp<E>::FR == 32) return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-	return 4 * r + (lane >> 4);
-}
+__device__ __forceinline__ int mm_col16(int lane, int r) { return std::is_same<E, double>::value ? 4 * r + (lane >> 4) : 4 * (lane >> 4) + r; }
 template <class E>
-__device__ __forceinline__ int mm_col16(int lane, int r) {
-	return std::is_same<E, double>::value ? 4 * r + (lane >> 4) : 4 * (lane >> 4) + r;
-}
+__device__ __forceinline__ int mm_col(int lane, int r) { return MmOp<E>::FR == 32 ? 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) : mm_col16<E>(lane, r); }
+template <class E> struct MmGroup { static constexpr int value = std::is_same<E, double>::value ? 1 : 4; };
 
 // exp, 1 / x and tanh for values that are rounded to T: 16-bit results take the instructions for 2^x and 1 / x (a relative error below 2^-20 for arguments up to 16,
 // a thousandth of a bf16 rounding, a hundredth of an fp16 one), fp32 and fp64 the full functions.
@@ -207,23 +198,37 @@ struct MmArgs {
 constexpr unsigned MM_OUT = 0x70000000u; // an offset behind every operand's end: such a load is answered with zeros
 constexpr int64_t MM_MAX_LD = 4 << 20;   // bytes: a tile's offsets (256 rows) stay within 2^30
 
-// E: operands, TM x TN: rows and columns (gated: TN / 2 columns of either projection) of a tile, WM x WN waves. DIRECT: operands whose rows begin
-// and end at multiples of 16 bytes go from global memory to LDS without registers; others are loaded a step ahead into registers.
-template <class E, int TM, int TN, int WM, int WN, bool GATED, bool DIRECT, class Epi>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >= 128 * 128 ? 1 : 2) void k_mm(MmArgs A, Epi epi) {
+// E: operands, TM x TN: rows and columns (gated: TN / 2 columns of either projection) of a tile, WM x WN waves, DEPTH steps in LDS. DIRECT: operands whose
+// rows begin and end at multiples of 16 bytes go from global memory to LDS without registers, DEPTH - 1 steps ahead; others are loaded a step ahead into
+// registers.
+template <class E_, int TM_, int TN_, int WM_, int WN_, int DEPTH_, bool GATED_, bool DIRECT_> struct MmShape {
+	typedef E_ E;
+	static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, DEPTH = DIRECT_ ? DEPTH_ : 2, THREADS = 64 * WM * WN;
+	static constexpr bool GATED = GATED_, DIRECT = DIRECT_;
+	static constexpr int NF = TN / WN / MmOp<E>::FR;
+	template <class Epi> static constexpr size_t lds() { // (the epilogue takes over what the steps have used)
+		const size_t steps = (size_t) DEPTH * (TM + TN) * 128, out = (size_t) WM * WN * Epi::template region<E, NF, GATED>();
+		return steps > out ? steps : out;
+	}
+};
+
 #ifdef __HIP_DEVICE_COMPILE__ // (the host pass knows no buffer descriptors)
-	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
+template <class Shape, class Epi>
+__device__ __forceinline__ void mm_tile(const MmArgs& A, const Epi& epi, unsigned block, unsigned blocks, char* mm_smem) {
+	typedef typename Shape::E E;
 	typedef MmOp<E> Op;
+	constexpr int TM = Shape::TM, TN = Shape::TN, WM = Shape::WM, WN = Shape::WN, DEPTH = Shape::DEPTH;
+	constexpr bool GATED = Shape::GATED, DIRECT = Shape::DIRECT;
 	constexpr int FR = Op::FR, NW = WM * WN, PIECES = 64 / FR, SUB = 8 / PIECES;
 	constexpr int SM = TM / WM, SN = TN / WN, MF = SM / FR, NF = SN / FR;
 	constexpr int LM = TM / 8 / NW, LN = TN / 8 / NW, BUF = (TM + TN) * 128;
-	static_assert(SUB % 2 == 0 && LM * 8 * NW == TM && LN * 8 * NW == TN && (!GATED || NF % 2 == 0), "tile");
+	static_assert(SUB % 2 == 0 && LM * 8 * NW == TM && LN * 8 * NW == TN && (!GATED || NF % 2 == 0) && (DEPTH & (DEPTH - 1)) == 0, "tile");
 	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
 
 	// Tiles go to the XCDs in runs (their L2s see neighbours), within a run 8 row tiles share each of the column tiles.
 	int tm, tn, part;
 	{
-		const unsigned n = gridDim.x, xcd = blockIdx.x % 8, at = blockIdx.x / 8, q = n / 8, rest = n % 8;
+		const unsigned xcd = block % 8, at = block / 8, q = blocks / 8, rest = blocks % 8;
 		unsigned t = xcd * q + min(xcd, rest) + at;
 		const unsigned per = (unsigned) A.tilesM * (unsigned) A.tilesN;
 		part = (int) (t / per);
@@ -254,10 +259,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 		if(GATED) rUp = __builtin_amdgcn_make_buffer_rsrc((void*) pUp, 0, colsIn * ldC, 0x00020000);
 	}
 	mm_i32x4 hold[DIRECT ? 1 : LM + LN];
-	auto issue = [&](int t, int which) { // step t's rows (1), columns (2): on their way to LDS (buffer t % 2), or into registers
+	auto issue = [&](int t, int which) { // step t's rows (1), columns (2): on their way to LDS (buffer t % DEPTH), or into registers
 		const int k = t * 128;
 		if(DIRECT) {
-			char* const to = mm_smem + (t & 1) * BUF;
+			char* const to = mm_smem + (t & (DEPTH - 1)) * BUF;
 			const bool out = k + piece >= K;
 			const unsigned vr = out ? MM_OUT : (unsigned) (lr * ldR + piece), vc = out ? MM_OUT : (unsigned) (lr * ldC + piece);
 #pragma unroll
@@ -304,7 +309,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 	mm_i32x4 fc[2][NF], fr[2][MF];
 	const int fl = (lane % FR) * 128;
 	auto read = [&](int set, int t, int s) {
-		const char* const from = mm_smem + (t & 1) * BUF + fl + (((s * PIECES + lane / FR) ^ ((lane % FR >> 1) & 7)) << 4);
+		const char* const from = mm_smem + (t & (DEPTH - 1)) * BUF + fl + (((s * PIECES + lane / FR) ^ ((lane % FR >> 1) & 7)) << 4);
 #pragma unroll
 		for(int j = 0; j < MF; j++) fr[set][j] = *(const mm_i32x4*) (from + (wm * SM + j * FR) * 128);
 #pragma unroll
@@ -317,15 +322,17 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 	};
 
 	if(nk > 0) {
-		issue(0, 3);
 		if(DIRECT) {
-			if(nk > 1) {
-				issue(1, 3);
-				asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LM + LN) : "memory");
-			}
+#pragma unroll
+			for(int t = 0; t < DEPTH; t++)
+				if(t < nk) issue(t, 3);
+			if(nk >= DEPTH) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * (LM + LN)) : "memory");
 			else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 		}
-		else put(0);
+		else {
+			issue(0, 3);
+			put(0);
+		}
 		barrier();
 		read(0, 0, 0);
 	}
@@ -334,14 +341,15 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 #pragma unroll
 		for(int s = 0; s < SUB; s++) {
 			// (a step's columns follow its rows a part of a step later: a wave cannot issue anything else while its copies wait in line)
-			if(DIRECT && s == 0 && t > 0 && t + 1 < nk) issue(t + 1, 2);
+			if(DIRECT && s == 0 && t > 0 && t + DEPTH - 1 < nk) issue(t + DEPTH - 1, 2);
 			if(s + 1 < SUB) read((s + 1) & 1, t, s + 1);
 			else if(t + 1 < nk) {
-				// everything of step t has been read; step t + 1 was requested a step ago
+				// everything of step t has been read; of the steps requested since, step t + 1 has to be there
 				if(DIRECT) {
-					asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+					if(DEPTH > 2 && t + DEPTH - 1 < nk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 2) * (LM + LN)) : "memory");
+					else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 					barrier();
-					if(t + 2 < nk) issue(t + 2, 1);
+					if(t + DEPTH < nk) issue(t + DEPTH, 1);
 				}
 				else {
 					put(t + 1); // (its buffer was last read in step t - 1)
@@ -352,7 +360,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 #pragma unroll
 			for(int i = 0; i < NF; i++)
 #pragma unroll
-				for(int j = 0; j < MF; j++) Op::mma(acc[i][j], fc[s & 1][i], fr[s & 1][j]);
+				for(int j = 0; j < MF; j++) {
+					if(sizeof(E) > 2 && s > 0 && t * 128 + s * PIECES * 16 >= K) continue; // (the last step's parts behind the operands' end: uniform)
+					Op::mma(acc[i][j], fc[s & 1][i], fr[s & 1][j]);
+				}
 			if(sizeof(E) <= 2) { // the next reads and copies between the products, not in front of them
 #pragma unroll
 				for(int q = 0; q < NF * MF; q++) {
@@ -365,6 +376,39 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 	}
 	barrier(); // LDS is the epilogue's
 	epi.template run<E, MF, NF, GATED>(acc, mm_smem + wave * Epi::template region<E, NF, GATED>(), m0 + wm * SM, n0 + wn * (GATED ? SN / 2 : SN), A.M, A.N, part, tm * WM + wm, lane);
+}
+#endif
+
+// 1: a wave to a SIMD and all its registers; the others leave room for two
+template <class Shape> constexpr int mm_waves() { return Shape::THREADS == 256 && Shape::TM * Shape::TN >= 256 * 256 ? 1 : 2; }
+
+template <class Shape, class Epi>
+__global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm(MmArgs A, Epi epi) {
+#ifdef __HIP_DEVICE_COMPILE__
+	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
+	mm_tile<Shape>(A, epi, blockIdx.x, gridDim.x, mm_smem);
+#endif
+}
+
+// A product and other work in one launch: blocks below `blocks` take its tiles, `more` gets the others, counted from 0.
+template <class Shape, class Epi, class More>
+__global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm_and(MmArgs A, Epi epi, unsigned blocks, More more) {
+#ifdef __HIP_DEVICE_COMPILE__
+	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
+	if(blockIdx.x < blocks) mm_tile<Shape>(A, epi, blockIdx.x, blocks, mm_smem);
+	else more.run(blockIdx.x - blocks, mm_smem);
+#endif
+}
+
+// Two products and other work in one launch.
+template <class Shape, class EpiA, class EpiB, class More>
+__global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm_two(MmArgs A, EpiA epiA, unsigned blocksA, MmArgs B, EpiB epiB, unsigned blocksB, More more) {
+#ifdef __HIP_DEVICE_COMPILE__
+	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
+	const unsigned b = blockIdx.x;
+	if(b < blocksA) mm_tile<Shape>(A, epiA, b, blocksA, mm_smem);
+	else if(b - blocksA < blocksB) mm_tile<Shape>(B, epiB, b - blocksA, blocksB, mm_smem);
+	else more.run(b - blocksA - blocksB, mm_smem);
 #endif
 }
 
@@ -373,6 +417,19 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN == 4 && TM * TN / (WM * WN) >
 // Lane: column (and row) lane % 16, 16 bytes from 16 (lane / 16) on of every 64. Rows that are not there are zeros. A turn's columns are requested a turn
 // ahead, the first ones in front of `before` (what has to be done before rowOf gives rows).
 constexpr int MMF_WAVES = 8, MMF_UNROLL = 4;
+// Whether that is faster than tiles: up to 16 rows, or so few results that tiles would leave most of the chip idle. In sixteens of rows times sixteens of columns, us
+// here / on tiles, K = 4096: bf16 gated 32 x 4096 (512) 19 / 30, 32 x 8192 (1024) 37 / 31, 64 x 4096 (1024) 26 / 31, 64 x 8192 (2048) 52 / 31; 8-bit 32 x 8192 (1024) 13 / 16,
+// 32 x 12288 (1536) 20 / 17, 37 x 7681 of K = 5001 (1443) 18 / 21, 64 x 4096 (1024) 12 / 16, 64 x 8192 (2048) 23 / 17; fp32 256 x 2048 (2048) 144 / 148, fp64 246 / 286, 512 x 2048 (4096) 280 / 154 and 487 / 288.
+template <class E>
+static inline bool mm_few_suits(int64_t m, int64_t n, int cus) {
+	return m <= 16 || (m + 15) / 16 * ((n + 15) / 16) <= (sizeof(E) == 1 ? 6 : sizeof(E) == 2 ? 4 : 8) * (int64_t) cus;
+}
+// How many rows (in sixteens) a block takes: up to 64, as few as it needs to give every CU one.
+static inline int mm_few_rows(int64_t m, int64_t n, int cus) {
+	for(int r = 4; r > 1; r >>= 1)
+		if(m > 8 * r && (m + 16 * r - 1) / (16 * r) * ((n + 15) / 16) >= cus) return r;
+	return 1;
+}
 template <class E, bool GATED, int MR, class Rows, class Before>
 __device__ __forceinline__ void mm_few(const char* cols, int64_t ldCols, int n0, int N, int64_t K, const Rows& rowOf, const Before& before,
 	typename MmOp<E>::Acc16 (&acc)[GATED ? 2 : 1][MR], int wave, int lane) {

@@ -16,7 +16,7 @@ __device__ __forceinline__ void mm_wave_sync() { // what the wave's lanes wrote 
 // The region: [half][row of the fragment][column], the halves of a gated unit apart.
 template <class E, int NF, bool GATED> struct MmRegion {
 	typedef typename MmOp<E>::Sum Sum;
-	static constexpr int FR = MmOp<E>::FR, H = GATED ? 2 : 1, COLS = NF * FR / H, R = FR * FR / 64, W = FR == 32 ? 4 : 1;
+	static constexpr int FR = MmOp<E>::FR, H = GATED ? 2 : 1, COLS = NF * FR / H, R = FR * FR / 64, W = MmGroup<E>::value;
 	static constexpr int PITCH = COLS * (int) sizeof(Sum) + 16, HALF = FR * PITCH, BYTES = H * HALF;
 	template <int MF, class Acc>
 	static __device__ __forceinline__ void put(char* region, Acc (&acc)[NF][MF], int j, int lane) {

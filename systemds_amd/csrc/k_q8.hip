@@ -217,7 +217,10 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_q8_few(Q8Few<T> A) {
 	extern __shared__ __attribute__((aligned(16))) char q8_smem[]; // sums: [wave][half][row][column]; FUSE: the 8-bit rows behind them
 	typedef typename MmCalc<T>::type C;
 	constexpr int H = GATED ? 2 : 1, SUMS = MMF_WAVES * H * MR * 1024;
-	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = blockIdx.x * 16;
+	const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MR;
+	if(!FUSE) { A.Q += m0 * A.ldQ; A.s += m0; }
+	A.out += m0 * A.ld;
+	A.m = min(A.m - m0, 16 * MR);
 	__shared__ float scales[FUSE ? Q8_FUSE : 1];
 	mm_i32x4 acc[H][MR];
 	const int pitch = (A.K + 15) & ~15;
@@ -303,8 +306,8 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_q8_few(Q8Few<T> A) {
 
 template <class T, bool GATED>
 static int q8_few(const Q8Few<T>& A, hipStream_t stream) {
-	const unsigned grid = (unsigned) ((A.N + 15) / 16);
-	const int MR = A.m <= 16 ? 1 : A.m <= 32 ? 2 : 4;
+	const int MR = A.Y ? 1 : mm_few_rows(A.m, A.N, g_numCU);
+	const dim3 grid((unsigned) ((A.N + 15) / 16), (unsigned) ((A.m + 16 * MR - 1) / (16 * MR)));
 	size_t lds = (size_t) MMF_WAVES * (GATED ? 2 : 1) * MR * 1024;
 	if(A.Y) {
 		lds += (size_t) A.m * ((A.K + 15) & ~15);
@@ -321,15 +324,14 @@ static int q8_few(const Q8Few<T>& A, hipStream_t stream) {
 	return 0;
 }
 
-template <class T, bool GATED, int TM, int TN>
+template <class T, bool GATED, int TM, int TN, int DEPTH = 2>
 static int q8_tile(MmArgs A, const MmEpiOut<T, true>& epi, hipStream_t stream) {
-	constexpr int WM = 2, WN = TM == 256 ? 4 : 2, NF = TN / WN / 32;
-	constexpr size_t lds = std::max(2 * (TM + TN) * 128, WM * WN * MmEpiOut<T, true>::template region<int8_t, NF, GATED>());
+	typedef MmShape<int8_t, TM, TN, 2, TM == 256 ? 4 : 2, DEPTH, GATED, true> Shape;
 	A.tilesM = (int32_t) ((A.M + TM - 1) / TM);
 	A.tilesN = (A.N + (GATED ? TN / 2 : TN) - 1) / (GATED ? TN / 2 : TN);
-	auto kernel = k_mm<int8_t, TM, TN, WM, WN, GATED, true, MmEpiOut<T, true>>;
+	auto kernel = k_mm<Shape, MmEpiOut<T, true>>;
 	CLA_HIP(allow_full_lds((const void*) kernel));
-	kernel<<<(unsigned) ((int64_t) A.tilesM * A.tilesN), 64 * WM * WN, lds, stream>>>(A, epi);
+	kernel<<<(unsigned) ((int64_t) A.tilesM * A.tilesN), Shape::THREADS, Shape::template lds<MmEpiOut<T, true>>(), stream>>>(A, epi);
 	CLA_HIP(hipGetLastError());
 	return 0;
 }
@@ -337,7 +339,7 @@ static int q8_tile(MmArgs A, const MmEpiOut<T, true>& epi, hipStream_t stream) {
 template <class T, bool GATED>
 static int q8_mm(const Q8Product& p, hipStream_t stream) {
 	const int N = GATED ? p.N / 2 : p.N; // columns of the output
-	if(p.m <= Q8_FEW)
+	if(mm_few_suits<int8_t>(p.m, N, g_numCU))
 		return q8_few<T, GATED>(Q8Few<T>{p.W, p.ldW, p.t, p.Q, p.ldQ, p.s, (int32_t) p.m, p.K, N, p.act, (const T*) p.bias, (T*) p.out, p.ldOut, (const T*) p.Y, p.ldY}, stream);
 	MmArgs A{};
 	A.rows = (const char*) p.Q; A.ldRows = p.ldQ;
@@ -348,6 +350,7 @@ static int q8_mm(const Q8Product& p, hipStream_t stream) {
 	const int64_t n = GATED ? 2 * (int64_t) N : N, big = ((p.m + 255) / 256) * ((n + 255) / 256), mid = ((p.m + 127) / 128) * ((n + 127) / 128);
 	if(big >= g_numCU) return q8_tile<T, GATED, 256, 256>(A, epi, stream);
 	if(mid >= g_numCU) return q8_tile<T, GATED, 128, 128>(A, epi, stream);
+	if(((p.m + 63) / 64) * ((n + 127) / 128) <= g_numCU) return q8_tile<T, GATED, 64, 128, 4>(A, epi, stream); // (a CU for itself: four steps in LDS)
 	return q8_tile<T, GATED, 64, 128>(A, epi, stream);
 }
 

@@ -5,7 +5,6 @@
 namespace cla {
 
 constexpr int Q8_MAX_K = 131071;  // terms of a sum: 128 * 128 * 131,071 < 2^31
-constexpr int Q8_FEW = 64;        // up to so many rows the product is a stream of the weights
 
 struct Q8Product {
 	const int8_t* W; int64_t ldW; const float* t;               // weights by column, their scales
