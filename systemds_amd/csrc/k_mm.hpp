@@ -414,7 +414,7 @@ __global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm_two(Mm
 
 // The same for few rows (up to 16 MR): columns are a stream of bytes that is read once, from global memory straight into the matrix operand. A block
 // takes 16 columns (gated: of either projection), its waves take turns of the summed index and add their sums up in LDS, in the order of the waves.
-// Lane: column (and row) lane % 16, 16 bytes from 16 (lane / 16) on of every 64. Rows that are not there are zeros. A turn's columns are requested a turn
+// Lane: column (and row) lane % 16, 16 bytes from 16 (lane / 16) on of every 64. Rows that are not there are zeros. A turn's columns are requested two turns
 // ahead, the first ones in front of `before` (what has to be done before rowOf gives rows).
 constexpr int MMF_WAVES = 8, MMF_UNROLL = 4;
 // Whether that is faster than tiles: up to 16 rows, or so few results that tiles would leave most of the chip idle. In sixteens of rows times sixteens of columns, us
@@ -466,14 +466,15 @@ __device__ __forceinline__ void mm_few(const char* cols, int64_t ldCols, int n0,
 		for(int j = 0; j < MR; j++) acc[h][j] = typename Op::Acc16{0, 0, 0, 0};
 	int64_t k = wave * TURN;
 	if(k < K) load(0, k);
+	if(k + STEP < K) load(1, k + STEP);
 	before();
 	while(k < K) { // (uniform)
-		if(k + STEP < K) load(1, k + STEP);
 		multiply(0, k);
+		if(k + 2 * STEP < K) load(0, k + 2 * STEP);
 		k += STEP;
 		if(k >= K) break;
-		if(k + STEP < K) load(0, k + STEP);
 		multiply(1, k);
+		if(k + 2 * STEP < K) load(1, k + 2 * STEP);
 		k += STEP;
 	}
 }

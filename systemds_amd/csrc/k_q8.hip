@@ -12,49 +12,77 @@ namespace cla {
 
 // ---- rows to 8 bits ----
 
-template <class T> struct Q8Most { static __device__ __forceinline__ float value() { return 3.4028234663852886e38f; } };
-template <> struct Q8Most<double> { static __device__ __forceinline__ double value() { return 1.7976931348623157e308; } };
+// Largest magnitude so far, with whatever is not finite above all that is. fp32: the bits without the sign, as a whole number.
+__device__ __forceinline__ uint32_t q8_more(float x, uint32_t m) { return max(m, __float_as_uint(x) & 0x7fffffffu); }
+__device__ __forceinline__ double q8_more(double x, double m) {
+	const double a = fabs(x);
+	return a <= 1.7976931348623157e308 ? fmax(a, m) : (double) INFINITY;
+}
+__device__ __forceinline__ float q8_value(uint32_t m) { return __uint_as_float(m); }
+__device__ __forceinline__ float q8_value(double m) { return (float) m; }
+
+// The scale of a row: the largest times 1 / 127, both in fp32. A row with a value that is not finite, or whose largest is none in fp32, has the scale NaN (and
+// zeros): its outputs are NaN.
+template <class M>
+__device__ __forceinline__ float q8_scale(M largest) {
+	const float a = q8_value(largest);
+	return a <= 3.4028234663852886e38f ? a * (1.0f / 127.0f) : NAN;
+}
+
+// What turns a row's values into whole numbers.
+template <class C> struct Q8Row {
+	C s, inv, half;
+	bool none, wide; // a row of zeros or one with the scale NaN; a scale whose reciprocal or last place leaves fp32's range
+	__device__ __forceinline__ explicit Q8Row(float scale) : s((C) scale), inv(C(1) / (C) scale), half(C(0.5) * (C) scale), none(!(scale > 0.0f)), wide(scale < 1e-30f) {}
+};
 
 // 16 bytes of a row (V values), `left` values of them there (the others 0)
 template <class T> struct Q8Piece {
 	static constexpr int V = 16 / (int) sizeof(T);
 	typedef typename MmCalc<T>::type C;
+	typedef typename std::conditional<std::is_same<C, double>::value, double, uint32_t>::type M;
+	struct Vals { T x[V]; };
 	static __device__ __forceinline__ mm_i32x4 load(const T* p, int64_t left) { return mm_load16<sizeof(T)>((const char*) p, left * (int) sizeof(T)); }
 	static __device__ __forceinline__ C value(const mm_i32x4& p, int v) { return (C) __builtin_bit_cast(Vals, p).x[v]; }
-	struct Vals { T x[V]; };
-	// largest magnitude; infinity where a value is none (infinite or NaN)
-	static __device__ __forceinline__ C largest(const mm_i32x4& p, C m) {
+	static __device__ __forceinline__ M largest(const mm_i32x4& p, M m) {
 #pragma unroll
-		for(int v = 0; v < V; v++) {
-			const C a = fabs(value(p, v));
-			m = a <= Q8Most<C>::value() ? (a > m ? a : m) : (C) INFINITY;
-		}
+		for(int v = 0; v < V; v++) m = q8_more(value(p, v), m);
 		return m;
 	}
+	// x / s to the nearest whole number r, ties to even, as the exact quotient rounds. Adding 1.5 * 2^23 (2^52) to x * (1 / s) leaves a number within one of it in
+	// the last bits. x - r s is exact next to s / 2 (both are multiples of x's or half of s's last place, below 2^24 or 2^53 of those): where it is below s / 2 in all
+	// of the piece, which is all but always, that is r. Otherwise the comparison decides value by value, and for scales out of range the quotient in fp64, whose
+	// distance from a half no fp32 operands can lose.
+	static __device__ __forceinline__ MmPack<int8_t, V> whole(const mm_i32x4& p, const Q8Row<C>& row) {
+		constexpr C BIG = std::is_same<C, double>::value ? C(6755399441055744.0) : C(12582912.0f);
+		MmPack<int8_t, V> o;
+		C far = C(0);
+#pragma unroll
+		for(int v = 0; v < V; v++) {
+			const C x = value(p, v), t = fma(x, row.inv, BIG), d = fma(BIG - t, row.s, x);
+			far = fmax(far, fabs(d));
+			o.x[v] = (int8_t) low(t);
+		}
+		if(far < row.half && !row.wide) return o;
+#pragma unroll
+		for(int v = 0; v < V; v++) {
+			const C x = value(p, v);
+			if(row.none) o.x[v] = 0;
+			else if(row.wide) o.x[v] = (int8_t) (int) fmin(fmax(rint((double) x / (double) row.s), -127.0), 127.0);
+			else {
+				C r = rint(x * row.inv);
+				const C d = fma(-r, row.s, x);
+				const bool odd = ((int) r & 1) != 0;
+				if(d > row.half || (d == row.half && odd)) r += C(1);
+				else if(d < -row.half || (d == -row.half && odd)) r -= C(1);
+				o.x[v] = (int8_t) (int) fmin(fmax(r, C(-127)), C(127));
+			}
+		}
+		return o;
+	}
+	static __device__ __forceinline__ uint32_t low(float t) { return __float_as_uint(t); }
+	static __device__ __forceinline__ uint32_t low(double t) { return (uint32_t) (unsigned long long) __double_as_longlong(t); }
 };
-
-// The scale of a row: the largest times 1 / 127, both in fp32. A row with a value that is not finite, or whose largest is none in fp32, has the scale NaN (and
-// zeros): its outputs are NaN.
-template <class C>
-__device__ __forceinline__ float q8_scale(C largest) {
-	const float a = (float) largest;
-	return a <= 3.4028234663852886e38f ? a * (1.0f / 127.0f) : NAN;
-}
-
-// x / s to the nearest whole number, ties to even, as the exact quotient rounds: the product with the reciprocal is within one of it, and x - r s is exact next to
-// s / 2 (both are multiples of x's or half of s's last place, below 2^24 or 2^53 of those), so comparing it with s / 2 decides. Scales whose reciprocal or
-// last place leaves the range take the quotient in fp64, whose distance from a half no fp32 operands can lose.
-template <class C>
-__device__ __forceinline__ int q8_round(C x, C s, C inv) {
-	C r = rint(x * inv);
-	const C d = fma(-r, s, x), half = C(0.5) * s;
-	const bool odd = ((int) r & 1) != 0;
-	if(d > half || (d == half && odd)) r += C(1);
-	else if(d < -half || (d == -half && odd)) r -= C(1);
-	return (int) fmin(fmax(r, C(-127)), C(127));
-}
-template <class C>
-__device__ __forceinline__ int q8_round_wide(C x, float s) { return (int) fmin(fmax(rint((double) x / (double) s), -127.0), 127.0); }
 
 // TPR threads to a row, NV pieces each, which stay in registers between the search for the largest and the rounding; longer rows are read again. Bound: a
 // row's bytes in and an eighth to a half of them out.
@@ -69,32 +97,30 @@ __global__ __launch_bounds__(256) void k_q8_rows(const T* __restrict__ Y, int64_
 	mm_i32x4 x[NV];
 #pragma unroll
 	for(int i = 0; i < NV; i++) x[i] = P::load(y + (i * TPR + t) * V, K - (i * TPR + t) * V);
-	C largest = C(0);
+	typename P::M largest = 0;
 #pragma unroll
 	for(int i = 0; i < NV; i++) largest = P::largest(x[i], largest);
 	for(int k = (NV * TPR + t) * V; k < K; k += TPR * V) largest = P::largest(P::load(y + k, K - k), largest);
 #pragma unroll
 	for(int d = (TPR < 64 ? TPR : 64) / 2; d > 0; d >>= 1) {
-		const C o = __shfl_xor(largest, d, 64);
+		const auto o = __shfl_xor(largest, d, 64);
 		largest = o > largest ? o : largest;
 	}
 	if(TPR > 64) {
-		__shared__ C part[4];
+		__shared__ typename P::M part[4];
 		if((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = largest;
 		__syncthreads();
 #pragma unroll
 		for(int i = 0; i < 4; i++) largest = part[i] > largest ? part[i] : largest;
 	}
 	if(row >= m) return;
-	const float s = q8_scale<C>(largest);
+	const float s = q8_scale(largest);
 	if(t == 0) scale[row] = s;
 	int8_t* const q = Q + row * ldQ;
-	const bool whole = (((uintptr_t) Q | (uintptr_t) ldQ) & (V - 1)) == 0, none = !(s > 0.0f), wide = s < 1e-30f;
-	const C inv = C(1) / (C) s;
+	const bool whole = (((uintptr_t) Q | (uintptr_t) ldQ) & (V - 1)) == 0;
+	const Q8Row<C> how(s);
 	auto put = [&](int k, const mm_i32x4& p) {
-		MmPack<int8_t, V> o;
-#pragma unroll
-		for(int v = 0; v < V; v++) o.x[v] = (int8_t) (none ? 0 : wide ? q8_round_wide<C>(P::value(p, v), s) : q8_round<C>(P::value(p, v), (C) s, inv));
+		const MmPack<int8_t, V> o = P::whole(p, how);
 		if(whole && k + V <= K) *(MmPack<int8_t, V>*) (q + k) = o;
 		else {
 #pragma unroll
@@ -104,7 +130,7 @@ __global__ __launch_bounds__(256) void k_q8_rows(const T* __restrict__ Y, int64_
 	};
 #pragma unroll
 	for(int i = 0; i < NV; i++)
-		if(i * TPR * V < K) put((i * TPR + t) * V, x[i]);
+		if(i == 0 || i * TPR * V < K) put((i * TPR + t) * V, x[i]);
 	for(int k = (NV * TPR + t) * V; k < K; k += TPR * V) put(k, P::load(y + k, K - k));
 }
 
@@ -113,17 +139,18 @@ static int q8_rows(const void* Yp, int64_t m, int K, int64_t ld, int8_t* Q, int6
 	if(m == 0) return 0;
 	constexpr int V = 16 / (int) sizeof(T);
 	const T* const Y = (const T*) Yp;
-	// Short rows 16 threads each, 16 rows a block; up to 8 pieces a lane a wave holds the row and no barrier is needed.
+	// Short rows 16 threads each, 16 rows a block; up to 2 pieces a lane a wave holds the row and no barrier is needed; longer ones take a block, few rows, too
+	// (idle waves would be all they leave).
 	const int64_t pieces = (K + V - 1) / V;
 #define Q8_ROWS(TPR, NV) k_q8_rows<T, TPR, NV><<<(unsigned) ((m + 256 / TPR - 1) / (256 / TPR)), 256, 0, stream>>>(Y, m, K, ld, Q, ldQ, scale)
 	if(pieces <= 16) Q8_ROWS(16, 1);
 	else if(pieces <= 64) Q8_ROWS(16, 4);
-	else if(m < 1024 || pieces > 64 * 8) {
-		if(pieces <= 512) Q8_ROWS(256, 2);
+	else if(m < 1024 || pieces > 64 * 2) {
+		if(pieces <= 256 * 2) Q8_ROWS(256, 2);
+		else if(pieces <= 256 * 4) Q8_ROWS(256, 4);
 		else Q8_ROWS(256, 8);
 	}
-	else if(pieces <= 64 * 2) Q8_ROWS(64, 2);
-	else Q8_ROWS(64, 8);
+	else Q8_ROWS(64, 2);
 #undef Q8_ROWS
 	CLA_HIP(hipGetLastError());
 	return 0;
@@ -228,44 +255,40 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_q8_few(Q8Few<T> A) {
 		if constexpr(FUSE) {
 			typedef Q8Piece<T> P;
 			constexpr int V = P::V, NV = 2, NT = 64 * MMF_WAVES;
-			__shared__ C part[Q8_FUSE][MMF_WAVES];
+			__shared__ typename P::M part[Q8_FUSE][MMF_WAVES];
 			mm_i32x4 x[Q8_FUSE][NV];
 #pragma unroll
-			for(int r = 0; r < Q8_FUSE; r++)
+			for(int r = 0; r < Q8_FUSE; r++) {
+				if(r >= A.m) break; // (uniform)
 #pragma unroll
-				for(int i = 0; i < NV; i++) x[r][i] = P::load(A.Y + min(r, A.m - 1) * A.ldY + (i * NT + tid) * V, r < A.m ? A.K - (i * NT + tid) * V : 0);
-			C big[Q8_FUSE];
+				for(int i = 0; i < NV; i++) x[r][i] = P::load(A.Y + r * A.ldY + (i * NT + tid) * V, A.K - (i * NT + tid) * V);
+			}
 #pragma unroll
 			for(int r = 0; r < Q8_FUSE; r++) {
-				big[r] = C(0);
+				if(r >= A.m) break;
+				typename P::M big = 0;
 #pragma unroll
-				for(int i = 0; i < NV; i++) big[r] = P::largest(x[r][i], big[r]);
-				if(r < A.m)
-					for(int k = (NV * NT + tid) * V; k < A.K; k += NT * V) big[r] = P::largest(P::load(A.Y + r * A.ldY + k, A.K - k), big[r]);
+				for(int i = 0; i < NV; i++) big = P::largest(x[r][i], big);
+				for(int k = (NV * NT + tid) * V; k < A.K; k += NT * V) big = P::largest(P::load(A.Y + r * A.ldY + k, A.K - k), big);
 #pragma unroll
 				for(int d = 32; d > 0; d >>= 1) {
-					const C o = __shfl_xor(big[r], d, 64);
-					big[r] = o > big[r] ? o : big[r];
+					const auto o = __shfl_xor(big, d, 64);
+					big = o > big ? o : big;
 				}
-				if(lane == 0) part[r][wave] = big[r];
+				if(lane == 0) part[r][wave] = big;
 			}
 			__syncthreads();
 #pragma unroll
 			for(int r = 0; r < Q8_FUSE; r++) {
 				if(r >= A.m) break;
-				C most = part[r][0];
+				typename P::M most = part[r][0];
 #pragma unroll
 				for(int w = 1; w < MMF_WAVES; w++) most = part[r][w] > most ? part[r][w] : most;
-				const float s = q8_scale<C>(most);
+				const float s = q8_scale(most);
 				if(tid == 0) scales[r] = s;
-				const bool none = !(s > 0.0f), wide = s < 1e-30f;
-				const C inv = C(1) / (C) s;
-				auto put = [&](int k, const mm_i32x4& p) { // (what lies behind the row is 0: so are the piece's bytes)
-					MmPack<int8_t, V> o;
-#pragma unroll
-					for(int v = 0; v < V; v++) o.x[v] = (int8_t) (none ? 0 : wide ? q8_round_wide<C>(P::value(p, v), s) : q8_round<C>(P::value(p, v), (C) s, inv));
-					*(MmPack<int8_t, V>*) (q8_smem + SUMS + r * pitch + k) = o;
-				};
+				const Q8Row<C> how(s);
+				// (what lies behind the row is 0: so are the piece's bytes)
+				auto put = [&](int k, const mm_i32x4& p) { *(MmPack<int8_t, V>*) (q8_smem + SUMS + r * pitch + k) = P::whole(p, how); };
 #pragma unroll
 				for(int i = 0; i < NV; i++)
 					if((i * NT + tid) * V < pitch) put((i * NT + tid) * V, x[r][i]);
