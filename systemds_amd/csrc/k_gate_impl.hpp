@@ -163,13 +163,10 @@ static MmArgs gate_args(const GateCall& c) {
 }
 
 template <class T>
-static bool whole(const void* p, int64_t ld) { return (((uintptr_t) p | (uintptr_t) (ld * (int64_t) sizeof(T))) & 15) == 0; }
-
-template <class T>
 int gate_forward(const GateCall& c, hipStream_t stream) {
 	if(mm_few_suits<T>(c.m, c.nOut, g_numCU))
 		return gate_few<T>(GateFew<T>{(const T*) c.Y, c.ldY, (const T*) c.W, c.ldW, (int32_t) c.m, c.nIn, c.nOut, c.act, (const T*) c.bias, (T*) c.out, c.ldOut}, stream);
-	const MmEpiOut<T, false> epi{nullptr, nullptr, (const T*) c.bias, (T*) c.out, c.ldOut, c.act, whole<T>(c.out, c.ldOut), 0};
+	const MmEpiOut<T, false> epi{nullptr, nullptr, (const T*) c.bias, (T*) c.out, c.ldOut, c.act, 0};
 	return gate_project<T>(gate_args<T>(c), epi, 0, GateNothing(), stream);
 }
 
@@ -200,12 +197,11 @@ template <class U> struct GateLayouts {
 		U* const dst = (U*) g.dst;
 		const int64_t r0 = (int64_t) (block % g.blocksR) * 64;
 		const int c0 = (int) (block / g.blocksR) * 64, a = threadIdx.x % PER * V, step = blockDim.x / PER;
-		const bool aligned = (((uintptr_t) src | (uintptr_t) (g.ld * sizeof(U))) & 15) == 0;
 		for(int b = threadIdx.x / PER; b < 64; b += step) {
 			MmPack<U, V> p;
 			const bool in = r0 + b < g.R;
 			const U* const from = src + (r0 + b) * g.ld + c0 + a;
-			if(in && aligned && c0 + a + V <= g.cols) p = *(const MmPack<U, V>*) from;
+			if(in && c0 + a + V <= g.cols) p = mm_get<MmPack<U, V>>(from);
 			else {
 #pragma unroll
 				for(int v = 0; v < V; v++) p.x[v] = in && c0 + a + v < g.cols ? from[v] : (U) 0;
@@ -315,9 +311,8 @@ template <class T> struct GateOut {
 		else part.template run<E, MF, NF, GATED>(acc, region, m0, n0, M, N, p, rowPart, lane);
 	}
 	static GateOut of(T* out, int64_t ld, typename MmCalc<T>::type* joins, int64_t M, int64_t N, int parts) {
-		typedef typename MmCalc<T>::type C;
-		return {{nullptr, nullptr, nullptr, out, ld, ACT_NONE, ::cla::whole<T>(out, ld), 0},
-			{nullptr, nullptr, nullptr, joins, N, ACT_NONE, ::cla::whole<C>(joins, N), M * N}, parts};
+		return {{nullptr, nullptr, nullptr, out, ld, ACT_NONE, 0},
+			{nullptr, nullptr, nullptr, joins, N, ACT_NONE, M * N}, parts};
 	}
 };
 
@@ -345,8 +340,7 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 
 	// projections, dG and dU; W and Y the other way round
 	const MmArgs project = gate_args<T>(c);
-	const MmEpiBack<T> back{(const T*) c.bias, (const T*) c.D, c.ldD, c.dY ? P : nullptr, 2 * p.half, c.dW ? Pt : nullptr, p.kPart, c.dB ? sums : nullptr, c.act,
-		whole<T>(c.D, c.ldD)};
+	const MmEpiBack<T> back{(const T*) c.bias, (const T*) c.D, c.ldD, c.dY ? P : nullptr, 2 * p.half, c.dW ? Pt : nullptr, p.kPart, c.dB ? sums : nullptr, c.act};
 	GateLayouts<U> lay{};
 	const int64_t one = (int64_t) 1 << 40; // (a single part)
 	if(c.dY)

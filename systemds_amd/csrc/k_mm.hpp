@@ -154,12 +154,32 @@ __device__ __forceinline__ void mm_act_both(C x, int act, C& value, C& slope) {
 	}
 }
 
-// 16 bytes of elements of ES bytes from any address of their alignment, `left` bytes of the row from there on: what lies behind the row is 0.
-template <int ES>
+// n consecutive values as one access
+template <class T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) MmPack { T x[N]; };
+// ... to or from an address that need not be a multiple of their size. (As whole words: a copy of values becomes an access for each.)
+template <int BYTES> struct MmWord { typedef mm_i32x4 type; };
+template <> struct MmWord<8> { typedef uint64_t type; };
+template <> struct MmWord<4> { typedef uint32_t type; };
+template <> struct MmWord<2> { typedef uint16_t type; };
+template <class P>
+__device__ __forceinline__ void mm_put(void* to, const P& p) {
+	const typename MmWord<sizeof(P)>::type w = __builtin_bit_cast(typename MmWord<sizeof(P)>::type, p);
+	__builtin_memcpy(to, &w, sizeof(P));
+}
+template <class P>
+__device__ __forceinline__ P mm_get(const void* from) {
+	typename MmWord<sizeof(P)>::type w;
+	__builtin_memcpy(&w, from, sizeof(P));
+	return __builtin_bit_cast(P, w);
+}
+
+// 16 bytes of elements of ES bytes from any address of their alignment, `left` bytes of the row from there on: what lies behind the row is 0. PARTIAL: rows
+// need not end at multiples of 16 bytes.
+template <int ES, bool PARTIAL = true>
 __device__ __forceinline__ mm_i32x4 mm_load16(const char* p, int64_t left) {
 	mm_i32x4 v = {0, 0, 0, 0};
 	if(left >= 16) __builtin_memcpy(&v, p, 16);
-	if(left > 0 && left < 16) { // (rare: behind a branch of its own, so that a lane's next loads do not wait for it)
+	if(PARTIAL && left > 0 && left < 16) { // (rare: behind a branch of its own, so that a lane's next loads do not wait for it)
 		if(ES == 8) { // (one of two)
 			uint64_t x;
 			__builtin_memcpy(&x, p, 8);
@@ -299,6 +319,8 @@ __device__ __forceinline__ void mm_tile(const MmArgs& A, const Epi& epi, unsigne
 	};
 
 	const int wm = wave % WM, wn = wave / WM;
+	constexpr int H = GATED ? 2 : 1;
+	const int fragments = H * ((A.N - n0 - wn * (SN / H) + FR - 1) / FR); // of the wave's columns that are there
 	typename Op::Acc acc[NF][MF];
 #pragma unroll
 	for(int i = 0; i < NF; i++)
@@ -361,7 +383,7 @@ __device__ __forceinline__ void mm_tile(const MmArgs& A, const Epi& epi, unsigne
 			for(int i = 0; i < NF; i++)
 #pragma unroll
 				for(int j = 0; j < MF; j++) {
-					if(sizeof(E) > 2 && s > 0 && t * 128 + s * PIECES * 16 >= K) continue; // (the last step's parts behind the operands' end: uniform)
+					if(sizeof(E) > 2 && ((s > 0 && t * 128 + s * PIECES * 16 >= K) || i >= fragments)) continue; // (what lies behind the operands' ends: uniform)
 					Op::mma(acc[i][j], fc[s & 1][i], fr[s & 1][j]);
 				}
 			if(sizeof(E) <= 2) { // the next reads and copies between the products, not in front of them
@@ -441,11 +463,11 @@ __device__ __forceinline__ void mm_few(const char* cols, int64_t ldCols, int n0,
 	const int c = min(n0 + l16, N - 1);
 	const char* const p[2] = {cols + (int64_t) c * ldCols + at, cols + ((int64_t) c + (GATED ? N : 0)) * ldCols + at};
 	mm_i32x4 w[2][H][U];
-	auto load = [&](int set, int64_t k) {
+	auto load = [&](int set, int64_t k) { // (8-bit weights are held in whole 128 bytes)
 #pragma unroll
 		for(int u = 0; u < U; u++)
 #pragma unroll
-			for(int h = 0; h < H; h++) w[set][h][u] = mm_load16<sizeof(E)>(p[h] + k + u * 64, K - (k + u * 64 + at));
+			for(int h = 0; h < H; h++) w[set][h][u] = mm_load16<sizeof(E), (sizeof(E) > 1)>(p[h] + k + u * 64, K - (k + u * 64 + at));
 	};
 	auto multiply = [&](int set, int64_t k) {
 		mm_i32x4 y[MR][U];

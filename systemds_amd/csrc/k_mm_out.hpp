@@ -5,9 +5,6 @@
 
 namespace cla {
 
-// n consecutive values as one access
-template <class T, int N> struct alignas(sizeof(T) * N > 16 ? 16 : sizeof(T) * N) MmPack { T x[N]; };
-
 __device__ __forceinline__ void mm_wave_sync() { // what the wave's lanes wrote to LDS is there for its other lanes
 	__builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 	__builtin_amdgcn_wave_barrier();
@@ -36,19 +33,15 @@ template <class E, int NF, bool GATED> struct MmRegion {
 	}
 };
 
-// V values to a row of the output, `cols` of them there
+// V values to a row of the output, `cols` of them there; 16 bytes at once wherever the row begins (value by value, as an address that is no multiple of 16 was served
+// before, 10,005 x 46 into 1716 in 8 bits took three times as long)
 template <class T, int V>
-__device__ __forceinline__ void mm_store(T* to, const T (&x)[V], int cols, bool aligned) {
-	if(aligned && cols >= V) {
-		MmPack<T, V> p;
-#pragma unroll
-		for(int v = 0; v < V; v++) p.x[v] = x[v];
-		*(MmPack<T, V>*) to = p;
-	}
+__device__ __forceinline__ void mm_store(T* to, const MmPack<T, V>& x, int cols) {
+	if(cols >= V) mm_put(to, x);
 	else {
 #pragma unroll
 		for(int v = 0; v < V; v++)
-			if(v < cols) to[v] = x[v];
+			if(v < cols) to[v] = x.x[v];
 	}
 }
 
@@ -61,7 +54,6 @@ template <class T, bool SCALED> struct MmEpiOut {
 	T* out;
 	int64_t ld;         // values
 	int32_t act;
-	int32_t aligned;    // out and its rows begin at multiples of 16 bytes
 	int64_t zOut;       // values between the outputs of the parts of the summed index
 
 	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
@@ -94,7 +86,7 @@ template <class T, bool SCALED> struct MmEpiOut {
 			for(int r0 = 0; r0 < FR; r0 += 64 / PER) {
 				const int r = r0 + lane / PER;
 				const C s = SCALED ? (C) __shfl(sr[j * FR / 64], (j * FR + r) & 63, 64) : C(1);
-				T x[V];
+				MmPack<T, V> x;
 #pragma unroll
 				for(int v = 0; v < V; v++) {
 					C y[H];
@@ -104,9 +96,9 @@ template <class T, bool SCALED> struct MmEpiOut {
 						if(SCALED) y[h] *= s * sc[h][v];
 						y[h] += bi[h][v];
 					}
-					x[v] = (T) (GATED ? mm_act<T>(y[0], act) * y[H - 1] : y[0]);
+					x.x[v] = (T) (GATED ? mm_act<T>(y[0], act) * y[H - 1] : y[0]);
 				}
-				if(row0 + r < M && cols > 0) mm_store<T, V>(out + part * zOut + (row0 + r) * ld + n0 + c, x, cols, aligned);
+				if(row0 + r < M && cols > 0) mm_store<T, V>(out + part * zOut + (row0 + r) * ld + n0 + c, x, cols);
 			}
 			mm_wave_sync();
 		}
@@ -127,7 +119,6 @@ template <class T> struct MmEpiBack {
 	int64_t kPart;      // a multiple of 256
 	C* sums;            // null: not wanted; [wave's rows][2 N]
 	int32_t act;
-	int32_t alignedD;
 
 	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
 	template <class E, int MF, int NF, bool GATED, class Acc>
@@ -155,9 +146,8 @@ template <class T> struct MmEpiBack {
 				const int r = r0 + lane / PER;
 				const bool in = row0 + r < M && c0 < cols;
 				const T* const d = D + (row0 + r) * ldD + n0 + c0;
-				T g[V], u[V];
-				MmPack<T, V> dv;
-				if(in && alignedD && c0 + V <= cols) dv = *(const MmPack<T, V>*) d;
+				MmPack<T, V> g, u, dv;
+				if(in && c0 + V <= cols) dv = mm_get<MmPack<T, V>>(d);
 				else {
 #pragma unroll
 					for(int v = 0; v < V; v++) dv.x[v] = in && c0 + v < cols ? d[v] : (T) 0.0f;
@@ -170,12 +160,12 @@ template <class T> struct MmEpiBack {
 					const bool there = in && c0 + v < cols;
 					const C dG = there ? (C) dv.x[v] * y * slope : C(0), dU = there ? (C) dv.x[v] * value : C(0);
 					*Reg::at(region, 0, r, c0 + v) = dG; *Reg::at(region, 1, r, c0 + v) = dU;
-					g[v] = (T) dG; u[v] = (T) dU;
+					g.x[v] = (T) dG; u.x[v] = (T) dU;
 				}
 				if(P && row0 + r < M && c0 < half) {
 					T* const to = P + (row0 + r) * ldP + n0 + c0;
-					mm_store<T, V>(to, g, V, true);
-					mm_store<T, V>(to + ldP / 2, u, V, true);
+					mm_store<T, V>(to, g, V);
+					mm_store<T, V>(to + ldP / 2, u, V);
 				}
 			}
 			mm_wave_sync();

@@ -117,11 +117,10 @@ __global__ __launch_bounds__(256) void k_q8_rows(const T* __restrict__ Y, int64_
 	const float s = q8_scale(largest);
 	if(t == 0) scale[row] = s;
 	int8_t* const q = Q + row * ldQ;
-	const bool whole = (((uintptr_t) Q | (uintptr_t) ldQ) & (V - 1)) == 0;
 	const Q8Row<C> how(s);
 	auto put = [&](int k, const mm_i32x4& p) {
 		const MmPack<int8_t, V> o = P::whole(p, how);
-		if(whole && k + V <= K) *(MmPack<int8_t, V>*) (q + k) = o;
+		if(k + V <= K) mm_put(q + k, o);
 		else {
 #pragma unroll
 			for(int v = 0; v < V; v++)
@@ -368,8 +367,7 @@ static int q8_mm(const Q8Product& p, hipStream_t stream) {
 	A.rows = (const char*) p.Q; A.ldRows = p.ldQ;
 	A.cols = (const char*) p.W; A.ldCols = p.ldW;
 	A.M = p.m; A.N = N; A.K = A.kPart = (p.K + 15) / 16 * 16; A.parts = 1;
-	const MmEpiOut<T, true> epi{p.s, p.t, (const T*) p.bias, (T*) p.out, p.ldOut, p.act,
-		(((uintptr_t) p.out | (uintptr_t) (p.ldOut * sizeof(T))) & 15) == 0, 0};
+	const MmEpiOut<T, true> epi{p.s, p.t, (const T*) p.bias, (T*) p.out, p.ldOut, p.act, 0};
 	const int64_t n = GATED ? 2 * (int64_t) N : N, big = ((p.m + 255) / 256) * ((n + 255) / 256), mid = ((p.m + 127) / 128) * ((n + 127) / 128);
 	if(big >= g_numCU) return q8_tile<T, GATED, 256, 256>(A, epi, stream);
 	if(mid >= g_numCU) return q8_tile<T, GATED, 128, 128>(A, epi, stream);
