@@ -23,7 +23,7 @@ GatePlan gate_plan(int type, int64_t m, int nIn, int nOut) {
 	const int64_t parts = gate_parts(2 * F, nIn, m * es / 128);
 	p.kPart = std::min((int64_t) up((size_t) ((std::max<int64_t>(m, 1) + parts - 1) / parts), 256), ((int64_t) 4 << 20) / es);
 	p.parts = (int32_t) std::max<int64_t>(1, (m + p.kPart - 1) / p.kPart);
-	p.sumRows = (int32_t) ((m + 31) / 32);
+	p.sumRows = (int32_t) ((m + 15) / 16);
 	p.sumJoins = (p.sumRows + 63) / 64;
 	size_t at = 0;
 	auto take = [&](int64_t bytes) { const size_t from = at; at += up((size_t) bytes, 256); return from; };

@@ -21,23 +21,26 @@ template <class T> struct GateFew {
 	int64_t ldY;
 	const T* W;
 	int64_t ldW;
-	int32_t m, nIn, nOut, act;
+	int64_t m;
+	int32_t nIn, nOut, act;
 	const T* bias;
 	T* out;
 	int64_t ld;
+	MmEpiBack<T> back;  // BACK: in place of out
 };
 
-// Few rows: a stream of the weights (k_mm.hpp); the sums of the block's waves meet in LDS.
-template <class T, int MR>
+// Few results: a stream of the weights (k_mm.hpp); the sums of the block's waves meet in LDS.
+template <class T, int MR, bool BACK>
 __global__ __launch_bounds__(64 * MMF_WAVES) void k_gate_few(GateFew<T> A) {
 	extern __shared__ __attribute__((aligned(16))) char gate_smem[]; // [wave][half][row][column]
 	typedef typename MmCalc<T>::type C;
 	typedef typename MmOp<T>::Acc16 Acc;
-	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MR;
-	A.Y += m0 * A.ldY; A.out += m0 * A.ld;
-	A.m = min(A.m - m0, 16 * MR);
+	const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16;
+	const int64_t m0 = (int64_t) blockIdx.y * 16 * MR;
+	const int rows = (int) min(A.m - m0, (int64_t) 16 * MR);
+	const T* const Y = A.Y + m0 * A.ldY;
 	Acc acc[2][MR];
-	auto rowOf = [&](int row, int64_t k, int64_t left) { return mm_load16<sizeof(T)>((const char*) (A.Y + (row < A.m ? row : 0) * A.ldY) + k, row < A.m ? left : 0); };
+	auto rowOf = [&](int row, int64_t k, int64_t left) { return mm_load16<sizeof(T)>((const char*) (Y + (row < rows ? row : 0) * A.ldY) + k, row < rows ? left : 0); };
 	mm_few<T, true, MR>((const char*) A.W, A.ldW * (int64_t) sizeof(T), n0, A.nOut, (int64_t) A.nIn * sizeof(T), rowOf, [] {}, acc, wave, lane);
 	C* const red = (C*) gate_smem;
 #pragma unroll
@@ -47,27 +50,63 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_gate_few(GateFew<T> A) {
 #pragma unroll
 			for(int r = 0; r < 4; r++) red[((wave * 2 + h) * MR * 16 + 16 * j + (lane & 15)) * 16 + mm_col16<T>(lane, r)] = acc[h][j][r];
 	__syncthreads();
-	for(int i = threadIdx.x; i < A.m * 16; i += 64 * MMF_WAVES) {
-		const int row = i >> 4, col = n0 + (i & 15);
-		if(col >= A.nOut) continue;
+	for(int i = threadIdx.x; i < (BACK ? 16 * MR : rows) * 16; i += 64 * MMF_WAVES) {
+		const int row = i >> 4, col = n0 + (i & 15), at = min(col, A.nOut - 1);
+		const bool in = row < rows && col < A.nOut;
 		C x[2];
 #pragma unroll
 		for(int h = 0; h < 2; h++) {
 			x[h] = C(0);
 #pragma unroll
 			for(int w = 0; w < MMF_WAVES; w++) x[h] += red[(w * 2 + h) * MR * 256 + i];
-			if(A.bias) x[h] += (C) A.bias[col + h * A.nOut];
+			if(A.bias) x[h] += (C) A.bias[at + h * A.nOut];
 		}
-		A.out[row * A.ld + col] = (T) (mm_act<T>(x[0], A.act) * x[1]);
+		if constexpr(!BACK) {
+			if(in) A.out[(m0 + row) * A.ld + col] = (T) (mm_act<T>(x[0], A.act) * x[1]);
+		}
+		else {
+			// (as MmEpiBack: zeros up to whole 16 bytes both ways)
+			const MmEpiBack<T>& B = A.back;
+			C value, slope;
+			mm_act_both<T>(x[0], A.act, value, slope);
+			const C d = in ? (C) B.D[(m0 + row) * B.ldD + col] : C(0);
+			const C dG = in ? d * x[1] * slope : C(0), dU = in ? d * value : C(0);
+			red[i] = dG; red[MR * 256 + i] = dU; // (of the first wave's sums nothing but this thread's are read at this place)
+			const int64_t half = B.ldP / 2, m = m0 + row, pad = 16 / (int) sizeof(T);
+			if(B.P && row < rows && col < half) {
+				B.P[m * B.ldP + col] = (T) dG;
+				B.P[m * B.ldP + half + col] = (T) dU;
+			}
+			if(B.Pt && col < A.nOut && m < (A.m + pad - 1) / pad * pad) {
+				const int64_t part = m / B.kPart;
+				T* const to = B.Pt + part * 2 * A.nOut * B.kPart + (m - part * B.kPart);
+				to[col * B.kPart] = (T) dG;
+				to[(col + A.nOut) * B.kPart] = (T) dU;
+			}
+		}
+	}
+	if constexpr(BACK) {
+		if(!A.back.sums) return; // (uniform)
+		__syncthreads();
+		const int h = threadIdx.x >> 4, c = threadIdx.x & 15;
+		if(h < 2 && n0 + c < A.nOut) {
+			C s = C(0);
+			for(int r = 0; r < rows; r++) s += red[h * MR * 256 + r * 16 + c];
+			A.back.sums[(int64_t) blockIdx.y * 2 * A.nOut + h * A.nOut + n0 + c] = s;
+		}
 	}
 }
 
+// Rows to a block, in sixteens (64 rows of fp64 do not fit the registers).
 template <class T>
+static int gate_few_rows(int64_t m, int nOut) { return std::min(mm_few_rows(m, nOut, g_numCU), sizeof(T) == 8 ? 2 : 4); }
+
+template <class T, bool BACK>
 static int gate_few(const GateFew<T>& A, hipStream_t stream) {
-	const int MR = std::min(mm_few_rows(A.m, A.nOut, g_numCU), sizeof(T) == 8 ? 2 : 4); // (64 rows of fp64 do not fit the registers)
+	const int MR = gate_few_rows<T>(A.m, A.nOut);
 	const dim3 grid((unsigned) ((A.nOut + 15) / 16), (unsigned) ((A.m + 16 * MR - 1) / (16 * MR)));
 	const size_t lds = (size_t) MMF_WAVES * 2 * MR * 256 * sizeof(typename MmCalc<T>::type);
-	auto kernel = MR == 1 ? k_gate_few<T, 1> : MR == 2 ? k_gate_few<T, 2> : k_gate_few<T, sizeof(T) == 8 ? 2 : 4>;
+	auto kernel = MR == 1 ? k_gate_few<T, 1, BACK> : MR == 2 ? k_gate_few<T, 2, BACK> : k_gate_few<T, sizeof(T) == 8 ? 2 : 4, BACK>;
 	if(lds > 65536) CLA_HIP(allow_full_lds((const void*) kernel));
 	kernel<<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
 	CLA_HIP(hipGetLastError());
@@ -165,7 +204,7 @@ static MmArgs gate_args(const GateCall& c) {
 template <class T>
 int gate_forward(const GateCall& c, hipStream_t stream) {
 	if(mm_few_suits<T>(c.m, c.nOut, g_numCU))
-		return gate_few<T>(GateFew<T>{(const T*) c.Y, c.ldY, (const T*) c.W, c.ldW, (int32_t) c.m, c.nIn, c.nOut, c.act, (const T*) c.bias, (T*) c.out, c.ldOut}, stream);
+		return gate_few<T, false>(GateFew<T>{(const T*) c.Y, c.ldY, (const T*) c.W, c.ldW, c.m, c.nIn, c.nOut, c.act, (const T*) c.bias, (T*) c.out, c.ldOut, {}}, stream);
 	const MmEpiOut<T, false> epi{nullptr, nullptr, (const T*) c.bias, (T*) c.out, c.ldOut, c.act, 0};
 	return gate_project<T>(gate_args<T>(c), epi, 0, GateNothing(), stream);
 }
@@ -350,12 +389,17 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 	// few of them behind the projections' tiles, in the same launch; many in one of their own: a tile's LDS leaves a CU to one block (4096 x 4096 into 2 x 8192 on
 	// bf16 1.85 ms in all, 1.49 so)
 	int64_t lays = (int64_t) lay.t[0].blocks + lay.t[1].blocks + lay.t[2].blocks;
-	if(lays > 2 * g_numCU) {
+	// (so few results that tiles would take a handful of CUs; more are written by column faster from a tile, and the layouts ride along: 59 x 4055 into 174 in fp64 277 us on
+	// tiles, 72 so, 76 x 256 into 2560 44 and 53)
+	const bool few = (c.m + 15) / 16 * ((F + 15) / 16) <= g_numCU;
+	if(lays > (few ? 0 : 2 * g_numCU)) {
 		if((rc = gate_grid(lays))) return rc;
 		k_gate_layouts<U><<<(unsigned) lays, 256, 0, stream>>>(lay);
 		lays = 0;
 	}
-	if((rc = gate_project<T>(project, back, lays, lay, stream))) return rc;
+	if(few) rc = gate_few<T, true>(GateFew<T>{(const T*) c.Y, c.ldY, (const T*) c.W, c.ldW, c.m, c.nIn, c.nOut, c.act, (const T*) c.bias, nullptr, 0, back}, stream);
+	else rc = gate_project<T>(project, back, lays, lay, stream);
+	if(rc) return rc;
 
 	// dY = P W and dW = t(P) Y; the first sums of dB
 	MmArgs A{}, B{};
@@ -367,7 +411,7 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 	C* const joinsY = (C*) (c.ws + p.joinsY);
 	C* const joinsW = (C*) (c.ws + p.joins);
 	const GateOut<T> outY = GateOut<T>::of((T*) c.dY, c.ldDY, joinsY, c.m, c.nIn, p.partsY), outW = GateOut<T>::of((T*) c.dW, c.ldDW, joinsW, 2 * F, c.nIn, p.parts);
-	const int waveRows = gate_shape<T>(project, true) / 1000 / 2, sumRows = (int) ((c.m + waveRows - 1) / waveRows); // (a row of partial sums per wave)
+	const int waveRows = few ? 16 * gate_few_rows<T>(c.m, c.nOut) : gate_shape<T>(project, true) / 1000 / 2, sumRows = (int) ((c.m + waveRows - 1) / waveRows); // (of a row of partial sums: a block's or a wave's)
 	GateSums<C> first{sums, sums64, sumRows, (int32_t) (2 * F), (sumRows + 63) / 64, (unsigned) ((2 * F + 63) / 64)};
 	MmArgs both = A; // (the shape that suits both: as many tiles as they have together)
 	both.M = A.M * A.parts + B.M * B.parts; both.parts = 1;
