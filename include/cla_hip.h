@@ -19,7 +19,7 @@
  * CG/ = C/colgroup/.
  *
  * Conventions
- *  - All matrices are dense row-major fp64 (Java DenseBlockFP64).
+ *  - All matrices are dense row-major fp64 (Java DenseBlockFP64), except where the products of layers below say their type.
  *  - Host pointers are borrowed only for the duration of the call.
  *  - `_dev` variants take device pointers (HBM) and run asynchronously on the
  *    block's stream up to the final non-zero count read-back; `_dev_async`
@@ -304,8 +304,8 @@ int cla_preagg(cla_handle h, int32_t group, const double* Y, int32_t nRowY, doub
 /* ---- products of layers: 8-bit matrices and gated units ----
  * What a network over the same data adds to the products above. Weights W are nRows x nCols as in Y %*% X: a row of Y has nRows values,
  * the output nCols. Operands and outputs are row-major with a leading dimension in elements, of one of the types below; device pointers are
- * aligned to their elements (int8 operands and workspaces to 16 bytes). Work is queued on a stream, nothing is allocated and nothing waited
- * for in the `_dev_async` forms, so that they can be captured into a graph; workspaces belong to the caller: calls that may run at the same
+ * aligned to their elements (8-bit rows of a product and workspaces to 16 bytes). Work is queued on a stream, nothing is allocated and nothing waited
+ * for in the `_dev_async` forms (but for a block's first cla_block_quantize_rows_dev_async), so that they can be captured into a graph; workspaces belong to the caller: calls that may run at the same
  * time (other streams, other graphs) take workspaces of their own. Operands, outputs and workspaces do not overlap. nRowY may be 0. */
 enum cla_type { CLA_F64 = 0, CLA_F32 = 1, CLA_BF16 = 2, CLA_F16 = 3 };
 /* Activations: 1 / (1 + exp(-x)), x / (1 + exp(-x)), x Phi(x), its tanh approximation, max(x, 0), x. */
@@ -316,11 +316,12 @@ enum cla_act { CLA_ACT_SIGMOID = 0, CLA_ACT_SILU = 1, CLA_ACT_GELU = 2, CLA_ACT_
  * The rows of dQ are ldQ bytes apart, of which the first k are written. No counterpart in the reference. Returns 0 or a negative error. */
 int cla_quantize_rows_dev_async(const void* dY, int32_t type, int64_t nRowY, int32_t k, int64_t ldY, int8_t* dQ, int64_t ldQ, float* dScale,
 	void* hipStream);
-/* The same for all rows of a compressed block, decoded in chunks (at most 64 MiB of scratch kept with the block) on its stream: what a layer with
- * many outputs takes instead of X %*% B. Returns 0 or a negative error without waiting for the stream. */
+/* The same for all rows of a compressed block, decoded in chunks on its stream: what a layer with many outputs takes instead of X %*% B. The first call
+ * allocates the chunk (at most 64 MiB, kept until the block is freed), so it is not the one to capture. Returns 0 or a negative error without waiting
+ * for the stream. */
 int cla_block_quantize_rows_dev_async(cla_handle h, int8_t* dQ, int64_t ldQ, float* dScale);
 
-/* An 8-bit matrix resident in HBM: W[k, j] = values[k, j] * scales[j]. nRows <= 131,071 (sums of products stay exact in 32 bits).
+/* An 8-bit matrix resident in HBM: W[k, j] = values[k, j] * scales[j]. nRows <= 131,071 (sums of products stay exact in 32 bits), nCols <= 2^21.
  * Calls on one handle are serialised, calls on different handles thread safe. */
 typedef struct cla_q8* cla_q8_handle;
 cla_q8_handle cla_q8_create(int64_t nRows, int32_t nCols);
@@ -359,12 +360,13 @@ int64_t cla_q8_gate(cla_q8_handle h, int32_t act, const double* Y, int64_t nRowY
 
 /* The gated unit in the operands' own type: out[nRowY x nOut] = act(Y %*% t(Wg) + bg) * (Y %*% t(Wu) + bu), W = rbind(Wg, Wu): 2 nOut x nIn, a row of
  * weights per output column; bias (2 nOut) may be null. 16-bit and fp32 operands are summed in fp32, fp64 in fp64. One kernel. At most 4 MiB a row
- * of Y and 1 MiB a row of the output. The workspace holds cla_gate_workspace(type, nRowY, nIn, nOut, 0) bytes (0: it may be null). */
+ * of Y and 1 MiB a row of the output, rows of Y and W at most 2 GiB apart. The workspace holds cla_gate_workspace(type, nRowY, nIn, nOut, 0) bytes (0: it may be null). */
 int64_t cla_gate_workspace(int32_t type, int64_t nRowY, int32_t nIn, int32_t nOut, int32_t backward);
 int cla_gate_dev_async(int32_t act, int32_t type, const void* dY, int64_t nRowY, int32_t nIn, int64_t ldY, const void* dW, int64_t ldW,
 	const void* dBias, int32_t nOut, void* dOut, int64_t ldOut, void* dWorkspace, int64_t workspaceBytes, void* hipStream);
 /* Its gradients from the incoming one (nRowY x nOut): of Y (nRowY x nIn), W (2 nOut x nIn) and bias (2 nOut); a null output is not computed. They
- * are written, not added to, and do not depend on timing. The projections are computed again; the workspace holds
+ * are written, not added to, and do not depend on timing. The projections are computed again; their gradients are rounded to `type` on the way to those
+ * of Y and W (fp16: infinite beyond 65504); the workspace holds
  * cla_gate_workspace(type, nRowY, nIn, nOut, 1) bytes. */
 int cla_gate_backward_dev_async(int32_t act, int32_t type, const void* dY, int64_t nRowY, int32_t nIn, int64_t ldY, const void* dW, int64_t ldW,
 	const void* dBias, int32_t nOut, const void* dGrad, int64_t ldGrad, void* dGradY, int64_t ldGradY, void* dGradW, int64_t ldGradW,

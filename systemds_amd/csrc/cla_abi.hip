@@ -345,6 +345,7 @@ void cla_block_free(cla_handle b) {
 	if(b->dStageIn) (void) hipFree(b->dStageIn);
 	if(b->dStageOut) (void) hipFree(b->dStageOut);
 	if(b->dScratch) (void) hipFree(b->dScratch);
+	if(b->dQuantRows) (void) hipFree(b->dQuantRows);
 	if(b->dChain) (void) hipFree(b->dChain);
 	if(b->dSdcPlan) (void) hipFree(b->dSdcPlan);
 	if(b->dSdcDesc) (void) hipFree(b->dSdcDesc);

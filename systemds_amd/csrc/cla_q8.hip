@@ -172,7 +172,7 @@ int cla_quantize_rows_dev_async(const void* dY, int32_t type, int64_t nRowY, int
 	const char* what = "quantize_rows";
 	int rc;
 	if((rc = check_type(what, type)) || (rc = check_rows(what, nRowY))) return rc;
-	if(k <= 0) { set_error("%s: rows of %d values", what, k); return -CLA_ERR_INVALID; }
+	if(k <= 0 || k > 1 << 30) { set_error("%s: rows of %d values", what, k); return -CLA_ERR_INVALID; } // (beyond 2^30 places in a row leave 32 bits)
 	if(nRowY == 0) return check_ready();
 	const size_t es = type_bytes(type);
 	if((rc = check_operand(what, "Y", dY, nRowY, k, ldY, es, es)) || (rc = check_operand(what, "the 8-bit rows", dQ, nRowY, k, ldQ, 1, 1)) ||
@@ -194,12 +194,12 @@ int cla_block_quantize_rows_dev_async(cla_handle b, int8_t* dQ, int64_t ldQ, flo
 	std::lock_guard<std::recursive_mutex> lk(b->mu);
 	clear_stats(b);
 	const int64_t bytes = (int64_t) b->nCols * 8, chunk = std::min<int64_t>(b->nRows, std::max<int64_t>(1, ((int64_t) 64 << 20) / bytes));
-	if((rc = ensure_scratch(b, (size_t) (chunk * bytes)))) return rc;
+	if(!b->dQuantRows) CLA_HIP(hipMalloc((void**) &b->dQuantRows, (size_t) (chunk * bytes)));
 	for(int64_t r0 = 0; r0 < b->nRows; r0 += chunk) {
 		const int64_t r1 = std::min(b->nRows, r0 + chunk);
-		if((rc = launch_decompress_rows(b, r0, r1, (double*) b->dScratch))) return rc;
+		if((rc = launch_decompress_rows(b, r0, r1, b->dQuantRows))) return rc;
 		Prof pf(b, "k_q8_rows", (long) (r1 - r0), 256, 0, (double) (r1 - r0) * (bytes + b->nCols + 4));
-		if((rc = launch_q8_rows(b->dScratch, CLA_F64, r1 - r0, b->nCols, b->nCols, dQ + r0 * ldQ, ldQ, dScale + r0, b->stream))) return rc;
+		if((rc = launch_q8_rows(b->dQuantRows, CLA_F64, r1 - r0, b->nCols, b->nCols, dQ + r0 * ldQ, ldQ, dScale + r0, b->stream))) return rc;
 	}
 	return 0;
 	CLA_CATCH_CODE(int)
@@ -208,8 +208,8 @@ int cla_block_quantize_rows_dev_async(cla_handle b, int8_t* dQ, int64_t ldQ, flo
 cla_q8_handle cla_q8_create(int64_t nRows, int32_t nCols) {
 	CLA_TRY
 	if(check_ready()) return nullptr;
-	if(nRows <= 0 || nCols <= 0 || nRows > Q8_MAX_K) {
-		set_error("invalid 8-bit matrix %lld x %d (at most %d rows)", (long long) nRows, nCols, Q8_MAX_K);
+	if(nRows <= 0 || nCols <= 0 || nRows > Q8_MAX_K || nCols > Q8_MAX_N) {
+		set_error("invalid 8-bit matrix %lld x %d (at most %d x %d)", (long long) nRows, nCols, Q8_MAX_K, Q8_MAX_N);
 		return nullptr;
 	}
 	cla_q8* h = new cla_q8();

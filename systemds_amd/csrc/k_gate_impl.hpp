@@ -6,7 +6,7 @@
 //   dY = [dG dU] [Wg; Wu],   dW = t([dG dU]) Y,   db = column sums of [dG dU]
 // together; then the sums that were split.
 // The tiles want both operands by rows of the summed index, so dG and dU are written by row and by column, W and Y are transposed into the workspace. dG and dU are
-// rounded to T between the products: the matrix cores take no wider operand, and a rounding of 2^-9 (bf16) of each of many terms leaves less than the result's own.
+// rounded to T between the products: the matrix cores take no wider operand, and a rounding of 2^-8 (bf16) of each of many terms leaves less than the result's own.
 // Sums over the batch for few weights are split into parts, joined in their order: results do not depend on timing.
 #pragma once
 #include "../../include/cla_hip.h"
@@ -387,7 +387,7 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 			lay.t[h] = GateTranspose::of((const T*) c.W + h * F * c.ldW, c.ldW, F, c.nIn, Wt + h * p.half, 2 * p.half, 0, p.half, one);
 	if(c.dW) lay.t[2] = GateTranspose::of(c.Y, c.ldY, c.m, c.nIn, Yt, p.kPart, c.nIn * p.kPart, pad, p.kPart);
 	// few of them behind the projections' tiles, in the same launch; many in one of their own: a tile's LDS leaves a CU to one block (4096 x 4096 into 2 x 8192 on
-	// bf16 1.85 ms in all, 1.49 so)
+	// bf16 1.85 ms in all, 1.50 so)
 	int64_t lays = (int64_t) lay.t[0].blocks + lay.t[1].blocks + lay.t[2].blocks;
 	// (so few results that tiles would take a handful of CUs; more are written by column faster from a tile, and the layouts ride along: 59 x 4055 into 174 in fp64 277 us on
 	// tiles, 72 so, 76 x 256 into 2560 44 and 53)

@@ -5,6 +5,7 @@
 namespace cla {
 
 constexpr int Q8_MAX_K = 131071;  // terms of a sum: 128 * 128 * 131,071 < 2^31
+constexpr int Q8_MAX_N = 1 << 21; // columns: 65,536 blocks of 32 where they are laid out
 
 struct Q8Product {
 	const int8_t* W; int64_t ldW; const float* t;               // weights by column, their scales

@@ -101,4 +101,33 @@ public final class ClaHipNative {
 	public static native int cooc(long h, int groupA, int groupB, long[] out);
 
 	public static native int preagg(long h, int group, double[] Y, int nRowY, double[] preAgg);
+
+	// ---- products of layers (no counterpart in the reference)
+
+	/** Activations of the gated units: 1 / (1 + exp(-x)), x / (1 + exp(-x)), x Phi(x), its tanh approximation, max(x, 0), x. */
+	public static final int ACT_SIGMOID = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_RELU = 4, ACT_NONE = 5;
+
+	/** cla_q8_create: an 8-bit matrix with a scale per column, resident on the device; 0 = not supported. */
+	public static native long q8Create(long nRows, int nCols);
+
+	public static native void q8Free(long h);
+
+	/** From dense fp64 (nRows x nCols), quantised column by column. */
+	public static native int q8Set(long h, double[] W);
+
+	/** From 8-bit values (nRows x nCols) and a scale per column, as they are. */
+	public static native int q8SetValues(long h, byte[] values, float[] scales);
+
+	/** out = Y %*% W (+ bias per column, may be null), rows of Y quantised in the call. */
+	public static native long q8Lmm(long h, double[] Y, long nRowY, double[] bias, double[] out);
+
+	/** out = act(Y %*% Wg) * (Y %*% Wu), Wg the first half of the columns, Wu the second. */
+	public static native long q8Gate(long h, int act, double[] Y, long nRowY, double[] bias, double[] out);
+
+	/** out = act(Y %*% t(Wg) + bg) * (Y %*% t(Wu) + bu), W = rbind(Wg, Wu). */
+	public static native long gate(int act, double[] Y, long nRowY, int nIn, double[] W, double[] bias, int nOut, double[] out);
+
+	/** Its gradients from the incoming one; a null output is not computed. */
+	public static native int gateBackward(int act, double[] Y, long nRowY, int nIn, double[] W, double[] bias, int nOut, double[] grad,
+		double[] gradY, double[] gradW, double[] gradBias);
 }

@@ -15,6 +15,7 @@
  */
 #include <jni.h>
 #include <stddef.h>
+#include <stdint.h>
 #include "cla_hip.h"
 
 #define FN(name) Java_org_apache_sysds_utils_ClaHipNative_##name
@@ -256,6 +257,107 @@ JNIEXPORT jint JNICALL FN(preagg)(JNIEnv* env, jclass c, jlong h, jint group, jd
 	double* p = pin(env, preAgg);
 	const jint rc = (y && p) ? cla_preagg(H(h), group, y, nRowY, p) : -CLA_ERR_INVALID;
 	unpin_out(env, preAgg, p);
+	unpin_in(env, Y, y);
+	return rc;
+}
+
+/* ---- products of layers ---- */
+#define Q(h) ((cla_q8_handle) (intptr_t) (h))
+
+JNIEXPORT jlong JNICALL FN(q8Create)(JNIEnv* env, jclass c, jlong nRows, jint nCols) {
+	(void) env; (void) c;
+	return (jlong) (intptr_t) cla_q8_create(nRows, nCols);
+}
+
+JNIEXPORT void JNICALL FN(q8Free)(JNIEnv* env, jclass c, jlong h) { (void) env; (void) c; cla_q8_free(Q(h)); }
+
+JNIEXPORT jint JNICALL FN(q8Set)(JNIEnv* env, jclass c, jlong h, jdoubleArray W) {
+	(void) c;
+	if(!holds(env, W, cla_q8_num_rows(Q(h)) * cla_q8_num_cols(Q(h)))) return -CLA_ERR_INVALID;
+	double* w = pin(env, W);
+	const jint rc = w ? cla_q8_set(Q(h), w) : -CLA_ERR_INVALID;
+	unpin_in(env, W, w);
+	return rc;
+}
+
+JNIEXPORT jint JNICALL FN(q8SetValues)(JNIEnv* env, jclass c, jlong h, jbyteArray values, jfloatArray scales) {
+	(void) c;
+	if(!holds(env, values, cla_q8_num_rows(Q(h)) * cla_q8_num_cols(Q(h))) || !holds(env, scales, cla_q8_num_cols(Q(h)))) return -CLA_ERR_INVALID;
+	jbyte* v = pin(env, values);
+	float* s = pin(env, scales);
+	const jint rc = (v && s) ? cla_q8_set_values(Q(h), (const int8_t*) v, s) : -CLA_ERR_INVALID;
+	unpin_in(env, scales, s);
+	unpin_in(env, values, v);
+	return rc;
+}
+
+/* products of an 8-bit matrix: nOut values to a row of the output */
+static jlong q8_product(JNIEnv* env, jlong h, int gated, jint act, jdoubleArray Y, jlong nRowY, jdoubleArray bias, jdoubleArray out) {
+	const jlong nR = cla_q8_num_rows(Q(h)), nC = cla_q8_num_cols(Q(h));
+	if(nRowY <= 0 || nR <= 0 || nRowY > INT32_MAX || !holds(env, Y, nRowY * nR) || (bias && !holds(env, bias, nC)) ||
+		!holds(env, out, nRowY * (gated ? nC / 2 : nC))) return -CLA_ERR_INVALID;
+	double* y = pin(env, Y);
+	double* b = pin(env, bias);
+	double* o = pin(env, out);
+	const jlong nnz = !y || !o || (bias && !b) ? -CLA_ERR_INVALID : gated ? cla_q8_gate(Q(h), act, y, nRowY, b, o) : cla_q8_lmm(Q(h), y, nRowY, b, o);
+	unpin_out(env, out, o);
+	unpin_in(env, bias, b);
+	unpin_in(env, Y, y);
+	return nnz;
+}
+
+JNIEXPORT jlong JNICALL FN(q8Lmm)(JNIEnv* env, jclass c, jlong h, jdoubleArray Y, jlong nRowY, jdoubleArray bias, jdoubleArray out) {
+	(void) c;
+	return q8_product(env, h, 0, 0, Y, nRowY, bias, out);
+}
+
+JNIEXPORT jlong JNICALL FN(q8Gate)(JNIEnv* env, jclass c, jlong h, jint act, jdoubleArray Y, jlong nRowY, jdoubleArray bias, jdoubleArray out) {
+	(void) c;
+	return q8_product(env, h, 1, act, Y, nRowY, bias, out);
+}
+
+/* sizes of a gated unit's arrays, products within 62 bits */
+static int gate_sizes(jlong nRowY, jint nIn, jint nOut) { return nRowY > 0 && nRowY <= INT32_MAX && nIn > 0 && nOut > 0 && nOut <= INT32_MAX / 2; }
+
+JNIEXPORT jlong JNICALL FN(gate)(JNIEnv* env, jclass c, jint act, jdoubleArray Y, jlong nRowY, jint nIn, jdoubleArray W, jdoubleArray bias, jint nOut,
+	jdoubleArray out) {
+	(void) c;
+	if(!gate_sizes(nRowY, nIn, nOut) || !holds(env, Y, nRowY * nIn) || !holds(env, W, 2 * (jlong) nOut * nIn) || (bias && !holds(env, bias, 2 * (jlong) nOut)) ||
+		!holds(env, out, nRowY * nOut)) return -CLA_ERR_INVALID;
+	double* y = pin(env, Y);
+	double* w = pin(env, W);
+	double* b = pin(env, bias);
+	double* o = pin(env, out);
+	const jlong nnz = (y && w && o && (!bias || b)) ? cla_gate(act, y, nRowY, nIn, w, b, nOut, o) : -CLA_ERR_INVALID;
+	unpin_out(env, out, o);
+	unpin_in(env, bias, b);
+	unpin_in(env, W, w);
+	unpin_in(env, Y, y);
+	return nnz;
+}
+
+JNIEXPORT jint JNICALL FN(gateBackward)(JNIEnv* env, jclass c, jint act, jdoubleArray Y, jlong nRowY, jint nIn, jdoubleArray W, jdoubleArray bias, jint nOut,
+	jdoubleArray grad, jdoubleArray gradY, jdoubleArray gradW, jdoubleArray gradBias) {
+	(void) c;
+	const jlong nW = 2 * (jlong) nOut * nIn;
+	if(!gate_sizes(nRowY, nIn, nOut) || !holds(env, Y, nRowY * nIn) || !holds(env, W, nW) || (bias && !holds(env, bias, 2 * (jlong) nOut)) ||
+		!holds(env, grad, nRowY * nOut) || (gradY && !holds(env, gradY, nRowY * nIn)) || (gradW && !holds(env, gradW, nW)) ||
+		(gradBias && !holds(env, gradBias, 2 * (jlong) nOut))) return -CLA_ERR_INVALID;
+	double* y = pin(env, Y);
+	double* w = pin(env, W);
+	double* b = pin(env, bias);
+	double* d = pin(env, grad);
+	double* gy = pin(env, gradY);
+	double* gw = pin(env, gradW);
+	double* gb = pin(env, gradBias);
+	const int there = y && w && d && (!bias || b) && (!gradY || gy) && (!gradW || gw) && (!gradBias || gb);
+	const jint rc = there ? cla_gate_backward(act, y, nRowY, nIn, w, b, nOut, d, gy, gw, gb) : -CLA_ERR_INVALID;
+	unpin_out(env, gradBias, gb);
+	unpin_out(env, gradW, gw);
+	unpin_out(env, gradY, gy);
+	unpin_in(env, grad, d);
+	unpin_in(env, bias, b);
+	unpin_in(env, W, w);
 	unpin_in(env, Y, y);
 	return rc;
 }

@@ -313,6 +313,60 @@ def test_rows_of_a_compressed_block(cla, ora):
     blk.close()
 
 
+def test_rows_of_a_compressed_block_captured(cla):
+    """... captured behind a first call, replayed when other products of the block have come and grown their own scratch."""
+    import ctypes as C
+
+    from conftest import mixed_block
+    lib, n_rows = hip(), 30011
+    specs, n_cols = mixed_block(4, n_rows)
+    blk = cla.build_block(n_rows, n_cols, specs)
+    stream, graph, run = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    assert lib.hipStreamCreate(C.byref(stream)) == 0
+    blk.set_stream(stream.value)
+    dQ, dS = DevBuf(n_rows * 32), DevBuf(4 * n_rows)
+    blk.quantize_rows_dev_async(dQ.ptr, 32, dS.ptr)
+    assert lib.hipStreamSynchronize(stream) == 0
+    want, scale = dQ.to_numpy((n_rows, 32), np.int8), dS.to_numpy(n_rows, np.float32)
+    assert lib.hipStreamBeginCapture(stream, 0) == 0
+    blk.quantize_rows_dev_async(dQ.ptr, 32, dS.ptr)
+    assert lib.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert lib.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)) == 0
+    for turn in range(3):
+        blk.aggregate("min", "row")
+        blk.tsmm()
+        assert lib.hipMemset(dQ.ptr, 0, dQ.nbytes) == 0 and lib.hipMemset(dS.ptr, 0, dS.nbytes) == 0
+        sync()
+        assert lib.hipGraphLaunch(run, stream) == 0
+        sync()
+        got = dQ.to_numpy((n_rows, 32), np.int8)
+        assert np.array_equal(got[:, :n_cols], want[:, :n_cols]) and np.array_equal(dS.to_numpy(n_rows, np.float32), scale)
+    assert lib.hipGraphExecDestroy(run) == 0 and lib.hipGraphDestroy(graph) == 0
+    blk.close()
+    assert lib.hipStreamDestroy(stream) == 0
+
+
+def test_two_threads_on_two_matrices(cla):
+    """Calls on two handles (streams of their own) from two threads, each checked against its own definition."""
+    import threading
+    cases = [Case(cla, 90, 300, 200, "bf16", seed=s) for s in (1, 2)]
+    errors = []
+
+    def work(c):
+        try:
+            for _ in range(10):
+                c.call()
+                c.check(c.result())
+        except BaseException as e:  # noqa: BLE001 - reported by the assertion below
+            errors.append(repr(e))
+    threads = [threading.Thread(target=work, args=(c,)) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+
+
 def test_captured_and_replayed(cla):
     """A call captured into a graph on a stream of its own, replayed with new rows in its buffers and eager calls of the same matrix between."""
     import ctypes as C
@@ -356,7 +410,7 @@ def test_refusals(cla):
         with pytest.raises(cla.ClaError, match=match) as e:
             f(*a, **k)
         assert e.value.code == code
-    for k, n in ((0, 4), (4, 0), (131072, 4)):
+    for k, n in ((0, 4), (4, 0), (131072, 4), (4, (1 << 21) + 1)):
         refused(-1, "invalid 8-bit matrix", cla.ClaQ8, k, n)
     h = cla.ClaQ8(20, 5)
     d = DevBuf(1 << 16)

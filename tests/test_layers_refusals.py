@@ -17,6 +17,7 @@ def test_quantize_rows():
     refused("-2 rows", f, p, 0, -2, 8, 8, p, 8, p)
     refused("2147483648 rows", f, p, 0, 1 << 31, 8, 8, p, 8, p)
     refused("rows of 0 values", f, p, 0, 3, 0, 8, p, 8, p)
+    refused("rows of 1073741825 values", f, p, 0, 3, (1 << 30) + 1, 1 << 31, p, 1 << 31, p)
     refused("Y is null", f, None, 0, 3, 8, 8, p, 8, p)
     refused("Y is not aligned", f, p + 4, 0, 3, 8, 8, p, 8, p)
     refused("leading dimension 7 of Y", f, p, 0, 3, 8, 7, p, 8, p)
