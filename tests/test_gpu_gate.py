@@ -248,6 +248,25 @@ def test_values_that_are_not_finite_stay_in_their_rows(cla, t, m):
     assert np.isnan(back[1]).all() and np.isnan(back[2]).all()
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m,n", [(5, 20), (100, 20), (1030, 1100), (2100, 2050)])
+def test_row_ends_inside_16_bytes(cla, t, m, n):
+    """What lies behind a row (the next row's first values, infinities and NaN here) stays out of its sums, in Y and in W, on every shape of tile and for every end."""
+    for k in (2 + 64, 3 + 64, 6 + 64, 31) if m < 1000 else (70,):
+        u = Unit(m, k, n, t, 1)
+        clean = u.forward().get()
+        u.Y[1::7, 0] = np.inf
+        u.W[3::50, 0] = np.nan
+        u.dY, u.dW = held(u.Y, t, k), held(u.W, t, k)
+        got = u.forward().get()
+        rows, cols = np.ones(m, bool), np.ones(n, bool)
+        rows[1::7] = False
+        bad = np.arange(3, 2 * n, 50)
+        cols[bad % n] = False
+        assert np.array_equal(got[np.ix_(rows, cols)], clean[np.ix_(rows, cols)])
+        assert np.isnan(got[:, ~cols]).all()
+
+
 def test_infinite_bias_beyond_the_batch(cla):
     """Rows that round the batch up are zeros in the sums whatever the bias is."""
     u = Unit(67, 24, 9, "bf16", 1)
