@@ -9,6 +9,11 @@
 // LDS rows are 128 bytes apart, half of its 64 banks; 16-byte piece c of row r lies at place c ^ (r / 2 % 8), so that 16 lanes that read one piece of 16
 // rows use every bank once (with r % 8 in its place half of the LDS cycles were conflicts). The copies to LDS write a wave's 1 KB in lane order: the
 // exchange is made in the addresses that the lanes read from.
+//
+// Bound: a step of a 256 x 256 tile has 2048 cycles of products on every SIMD next to 192 KB of LDS reads by eight waves of 128 x 64 and 64 KB of copies (four waves of 128 x 128 read
+// 128 KB, but a wave alone on its SIMD leaves it idle at every wait: bf16 8192 x 8192 x 8192 895 us, eight waves 820 = 1.34 PFLOP/s at 1.82 GHz, 71 % of the cycles in products).
+// Smaller tiles are bound by LDS (64 x 128: 48 KB of reads for 256 cycles of products) and are for fewer results than fill the chip. fp32 and fp64 are bound by their
+// matrix instructions at any size (16 x 16 x 4: 32 and 64 cycles).
 #pragma once
 #include "cla_device.hpp"
 

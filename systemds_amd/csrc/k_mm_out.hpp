@@ -33,8 +33,7 @@ template <class E, int NF, bool GATED> struct MmRegion {
 	}
 };
 
-// V values to a row of the output, `cols` of them there; 16 bytes at once wherever the row begins (value by value, as an address that is no multiple of 16 was served
-// before, 10,005 x 46 into 1716 in 8 bits took 59 us and not 32)
+// V values to a row of the output, `cols` of them there: 16 bytes at once wherever the row begins.
 template <class T, int V>
 __device__ __forceinline__ void mm_store(T* to, const MmPack<T, V>& x, int cols) {
 	if(cols >= V) mm_put(to, x);
