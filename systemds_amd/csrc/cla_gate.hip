@@ -179,7 +179,7 @@ int64_t cla_gate(int32_t act, const double* Y, int64_t nRowY, int32_t nIn, const
 	if(nRowY == 0) return 0;
 	const size_t nY = (size_t) nRowY * nIn, nW = 2 * (size_t) nOut * nIn, nB = bias ? 2 * (size_t) nOut : 0, nO = (size_t) nRowY * nOut;
 	GateStage s;
-	CLA_HIP(hipMalloc((void**) &s.p, (nY + nW + nB + nO + 1) * 8 + 5 * 256));
+	if((rc = device_room("gate", (void**) &s.p, (nY + nW + nB + nO + 1) * 8 + 5 * 256))) return rc;
 	double* const y = s.take(nY);
 	double* const w = s.take(nW);
 	double* const b = s.take(nB);
@@ -205,7 +205,7 @@ int cla_gate_backward(int32_t act, const double* Y, int64_t nRowY, int32_t nIn, 
 	const size_t nY = (size_t) nRowY * nIn, nW = 2 * (size_t) nOut * nIn, nB = 2 * (size_t) nOut, nO = (size_t) nRowY * nOut;
 	const int64_t wsBytes = cla_gate_workspace(CLA_F64, nRowY, nIn, nOut, 1);
 	GateStage s;
-	CLA_HIP(hipMalloc((void**) &s.p, (2 * nY + 2 * nW + 2 * nB + nO) * 8 + 8 * 256 + (size_t) wsBytes));
+	if((rc = device_room("gate_backward", (void**) &s.p, (2 * nY + 2 * nW + 2 * nB + nO) * 8 + 8 * 256 + (size_t) wsBytes))) return rc;
 	double* const y = s.take(nY);
 	double* const w = s.take(nW);
 	double* const b = s.take(nB);

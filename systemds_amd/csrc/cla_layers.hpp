@@ -11,6 +11,8 @@ int check_act(const char* what, int act);
 int check_rows(const char* what, int64_t m);
 // A row-major operand: there, aligned to `to` bytes, rows that do not overlap, its bytes within 63 bits.
 int check_operand(const char* what, const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld, size_t es, size_t to);
+// Device memory for a call; where there is none, the runtime's error does not stay for the next call to find.
+int device_room(const char* what, void** p, size_t bytes);
 // Non-zeros of n values on the device; waits for the stream.
 int64_t count_nonzero(const double* x, int64_t n, unsigned long long* dCount, hipStream_t stream);
 

@@ -48,6 +48,12 @@ int check_rows(const char* what, int64_t m) {
 	return -CLA_ERR_INVALID;
 }
 
+int device_room(const char* what, void** p, size_t bytes) {
+	if(!no_room(p, bytes)) return 0;
+	set_error("%s: %zu bytes of device memory could not be allocated", what, bytes);
+	return -CLA_ERR_DEVICE;
+}
+
 __global__ __launch_bounds__(256) void k_count_nonzero(const double* __restrict__ x, int64_t n, unsigned long long* __restrict__ count) {
 	unsigned long long c = 0;
 	for(int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) c += x[i] != 0.0;
@@ -148,7 +154,7 @@ static int64_t host_product(cla_q8* h, const char* what, bool gated, int act, co
 	if(need > h->stageCap) {
 		if(h->dStage) CLA_HIP(hipFree(h->dStage)); // (no call of a host form is under way)
 		h->dStage = nullptr; h->stageCap = 0;
-		CLA_HIP(hipMalloc(&h->dStage, need));
+		if(int r = device_room(what, &h->dStage, need)) return r;
 		h->stageCap = need;
 	}
 	char* const base = (char*) h->dStage;
@@ -194,7 +200,7 @@ int cla_block_quantize_rows_dev_async(cla_handle b, int8_t* dQ, int64_t ldQ, flo
 	std::lock_guard<std::recursive_mutex> lk(b->mu);
 	clear_stats(b);
 	const int64_t bytes = (int64_t) b->nCols * 8, chunk = std::min<int64_t>(b->nRows, std::max<int64_t>(1, ((int64_t) 64 << 20) / bytes));
-	if(!b->dQuantRows) CLA_HIP(hipMalloc((void**) &b->dQuantRows, (size_t) (chunk * bytes)));
+	if(!b->dQuantRows && (rc = device_room(what, (void**) &b->dQuantRows, (size_t) (chunk * bytes)))) return rc;
 	for(int64_t r0 = 0; r0 < b->nRows; r0 += chunk) {
 		const int64_t r1 = std::min(b->nRows, r0 + chunk);
 		if((rc = launch_decompress_rows(b, r0, r1, b->dQuantRows))) return rc;
@@ -264,7 +270,7 @@ int cla_q8_set_dev(cla_q8_handle h, const void* dW, int32_t type, int64_t ld, in
 	DevTmp tmp;
 	if(byColumn) rc = launch_q8_rows(dW, type, h->nCols, (int) h->nRows, ld, h->dW, h->ldW, h->dScale, h->stream);
 	else {
-		CLA_HIP(hipMalloc(&tmp.p, (size_t) h->nRows * h->nCols * 8));
+		if((rc = device_room(what, &tmp.p, (size_t) h->nRows * h->nCols * 8))) return rc;
 		rc = launch_q8_columns(dW, type, ld, h->nRows, h->nCols, (double*) tmp.p, h->stream);
 		if(!rc) rc = launch_q8_rows(tmp.p, CLA_F64, h->nCols, (int) h->nRows, h->nRows, h->dW, h->ldW, h->dScale, h->stream);
 	}
@@ -284,7 +290,7 @@ int cla_q8_set(cla_q8_handle h, const double* W) {
 	std::lock_guard<std::recursive_mutex> lk(h->mu);
 	DevTmp tmp;
 	const size_t bytes = (size_t) h->nRows * h->nCols * 8;
-	CLA_HIP(hipMalloc(&tmp.p, bytes));
+	if((rc = device_room("q8_set", &tmp.p, bytes))) return rc;
 	CLA_HIP(hipMemcpyAsync(tmp.p, W, bytes, hipMemcpyHostToDevice, h->stream));
 	rc = cla_q8_set_dev(h, tmp.p, CLA_F64, h->nCols, 0);
 	(void) hipStreamSynchronize(h->stream);
@@ -316,8 +322,7 @@ int cla_q8_set_values(cla_q8_handle h, const int8_t* values, const float* scales
 	std::lock_guard<std::recursive_mutex> lk(h->mu);
 	DevTmp v, s;
 	const size_t n = (size_t) h->nRows * h->nCols;
-	CLA_HIP(hipMalloc(&v.p, n));
-	CLA_HIP(hipMalloc(&s.p, sizeof(float) * (size_t) h->nCols));
+	if((rc = device_room("q8_set_values", &v.p, n)) || (rc = device_room("q8_set_values", &s.p, sizeof(float) * (size_t) h->nCols))) return rc;
 	CLA_HIP(hipMemcpyAsync(v.p, values, n, hipMemcpyHostToDevice, h->stream));
 	CLA_HIP(hipMemcpyAsync(s.p, scales, sizeof(float) * (size_t) h->nCols, hipMemcpyHostToDevice, h->stream));
 	rc = cla_q8_set_values_dev(h, (const int8_t*) v.p, h->nCols, 0, (const float*) s.p);

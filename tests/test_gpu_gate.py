@@ -175,6 +175,55 @@ def test_rows_apart(cla, t, m):
     u.check_backward(u.backward())
 
 
+class Shifted:
+    """A copy of a device buffer that begins one element behind an aligned address."""
+
+    def __init__(self, buf, t):
+        raw = np.concatenate([np.zeros(BYTES[t], np.uint8), buf.to_numpy(buf.nbytes, np.uint8)])
+        self.buf = DevBuf.from_numpy(raw)
+        self.ptr = self.buf.ptr + BYTES[t]
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("m", [3, 90, 700])
+def test_operands_at_odd_places(cla, t, m):
+    """Operands, biases and the incoming gradient one element behind an aligned address; outputs, too."""
+    u = Unit(m, 96, 40, t, m)
+    for name in ("dY", "dW", "dD", "dB"):
+        setattr(u, name, Shifted(getattr(u, name), t))
+    u.check_forward(u.forward().get())
+    u.check_backward(u.backward())
+    from systemds_amd import capi
+    want = u.forward().get()
+    odd = DevBuf(m * 40 * BYTES[t] + 64)
+    capi.gate_dev_async(*u.args(), odd.ptr + BYTES[t], 40)
+    sync()
+    raw = odd.to_numpy(odd.nbytes, np.uint8)[BYTES[t]:BYTES[t] * (1 + m * 40)].copy()
+    assert np.array_equal(decode(raw.view(encode(np.zeros(0), t).dtype).reshape(m, 40), t), want)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_two_streams_at_once(cla, t):
+    """The gradients of two units queued on two streams, each with a workspace of its own, several times over."""
+    import ctypes as C
+    from systemds_amd import capi
+    lib, streams, units = hip(), [C.c_void_p(), C.c_void_p()], []
+    for i, s in enumerate(streams):
+        assert lib.hipStreamCreate(C.byref(s)) == 0
+        u = Unit(900, 130, 70, t, i + 1)
+        u.got = u.backward()  # (allocates)
+        units.append(u)
+    need = capi.gate_workspace(TYPE_IDS[t], 900, 130, 70, True)
+    for _ in range(6):
+        for u, s in zip(units, streams):
+            o = u.got
+            capi.gate_backward_dev_async(*u.args(), u.dD.ptr, 70, o[0].buf.ptr, 130, o[1].buf.ptr, 130, o[2].buf.ptr, u.ws.ptr, need, s.value)
+    sync()
+    for u, s in zip(units, streams):
+        u.check_backward(u.got)
+        assert lib.hipStreamDestroy(s) == 0
+
+
 @pytest.mark.parametrize("t,m,k,n", [("bf16", 2100, 256, 2048), ("f16", 4100, 136, 1100), ("f64", 2050, 70, 2049), ("f32", 2050, 72, 2050)])
 def test_large_tiles(cla, t, m, k, n):
     u = Unit(m, k, n, t, 3)
