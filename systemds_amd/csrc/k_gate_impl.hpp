@@ -110,7 +110,8 @@ static int gate_few(const GateFew<T>& A, hipStream_t stream) {
 	const int MR = gate_few_rows<T>(A.m, A.nOut);
 	const dim3 grid((unsigned) ((A.nOut + 15) / 16), (unsigned) ((A.m + 16 * MR - 1) / (16 * MR)));
 	const size_t lds = (size_t) MMF_WAVES * 2 * MR * 256 * sizeof(typename MmCalc<T>::type);
-	auto kernel = MR == 1 ? k_gate_few<T, 1, BACK> : MR == 2 ? k_gate_few<T, 2, BACK> : k_gate_few<T, sizeof(T) == 8 ? 2 : 4, BACK>;
+	constexpr bool WIDE = sizeof(T) == 8;
+	auto kernel = MR == 1 ? k_gate_few<T, 1, BACK> : MR == 2 ? k_gate_few<T, 2, BACK> : MR == 3 ? k_gate_few<T, WIDE ? 2 : 3, BACK> : k_gate_few<T, WIDE ? 2 : 4, BACK>;
 	if(lds > 65536) CLA_HIP(allow_full_lds((const void*) kernel));
 	kernel<<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
 	CLA_HIP(hipGetLastError());

@@ -170,15 +170,23 @@ int launch_q8_rows(const void* Y, int type, int64_t m, int K, int64_t ld, int8_t
 
 // ---- weights: a column's values one after the other, zeros up to a multiple of 128 ----
 
-// byColumn: the source has a row per column already
-__global__ __launch_bounds__(256) void k_q8_layout(const int8_t* __restrict__ src, int64_t ld, int byColumn, int64_t K, int N, int8_t* __restrict__ W, int64_t ldW) {
+// The source has a row per column already: 16 bytes a thread (4096 x 4096 147 us value by value, 12 so).
+__global__ __launch_bounds__(256) void k_q8_pad(const int8_t* __restrict__ src, int64_t ld, int64_t K, int64_t N, int8_t* __restrict__ W, int64_t ldW) {
+	const int64_t per = ldW / 16, n = N * per;
+	for(int64_t i = (int64_t) blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t) gridDim.x * 256) {
+		const int64_t col = i / per, k = i % per * 16;
+		*(mm_i32x4*) (W + col * ldW + k) = mm_load16<1>((const char*) src + col * ld + k, K - k);
+	}
+}
+
+// The source is row-major: 64 x 64 values through LDS.
+__global__ __launch_bounds__(256) void k_q8_layout(const int8_t* __restrict__ src, int64_t ld, int64_t K, int N, int8_t* __restrict__ W, int64_t ldW) {
 	__shared__ int8_t tile[64][65];
 	const int64_t k0 = (int64_t) blockIdx.x * 64;
 	const int n0 = blockIdx.y * 64;
 	for(int i = threadIdx.x; i < 4096; i += 256) {
 		const int a = i >> 6, b = i & 63;
-		if(byColumn) tile[a][b] = n0 + a < N && k0 + b < K ? src[(int64_t) (n0 + a) * ld + k0 + b] : (int8_t) 0;
-		else tile[b][a] = n0 + b < N && k0 + a < K ? src[(k0 + a) * ld + n0 + b] : (int8_t) 0;
+		tile[b][a] = n0 + b < N && k0 + a < K ? src[(k0 + a) * ld + n0 + b] : (int8_t) 0;
 	}
 	__syncthreads();
 	for(int i = threadIdx.x; i < 4096; i += 256) {
@@ -188,7 +196,8 @@ __global__ __launch_bounds__(256) void k_q8_layout(const int8_t* __restrict__ sr
 }
 
 int launch_q8_layout(const int8_t* src, int64_t ld, int byColumn, int64_t K, int N, int8_t* W, int64_t ldW, hipStream_t stream) {
-	k_q8_layout<<<dim3((unsigned) (ldW / 64), (unsigned) ((N + 63) / 64)), 256, 0, stream>>>(src, ld, byColumn, K, N, W, ldW);
+	if(byColumn) k_q8_pad<<<(unsigned) std::min<int64_t>((ldW / 16 * N + 255) / 256, (int64_t) g_numCU * 16), 256, 0, stream>>>(src, ld, K, N, W, ldW);
+	else k_q8_layout<<<dim3((unsigned) (ldW / 64), (unsigned) ((N + 63) / 64)), 256, 0, stream>>>(src, ld, K, N, W, ldW);
 	CLA_HIP(hipGetLastError());
 	return 0;
 }
@@ -342,6 +351,7 @@ static int q8_few(const Q8Few<T>& A, hipStream_t stream) {
 	}
 	else if(MR == 1) k_q8_few<T, GATED, 1, false><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
 	else if(MR == 2) k_q8_few<T, GATED, 2, false><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
+	else if(MR == 3) k_q8_few<T, GATED, 3, false><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
 	else {
 		CLA_HIP(allow_full_lds((const void*) k_q8_few<T, GATED, 4, false>));
 		k_q8_few<T, GATED, 4, false><<<grid, 64 * MMF_WAVES, lds, stream>>>(A);
