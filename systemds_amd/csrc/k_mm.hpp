@@ -225,8 +225,7 @@ constexpr int64_t MM_MAX_LD = 4 << 20;   // bytes: a tile's offsets (256 rows) s
 
 // E: operands, TM x TN: rows and columns (gated: TN / 2 columns of either projection) of a tile, WM x WN waves, DEPTH steps in LDS. DIRECT: operands whose
 // rows begin and end at multiples of 4 bytes go from global memory to LDS without registers, DEPTH - 1 steps ahead (what a row's last 16 bytes hold of the next
-// row is cleared in LDS); others are loaded a step ahead into
-// registers.
+// row is cleared in LDS); others are loaded a step ahead into registers.
 template <class E_, int TM_, int TN_, int WM_, int WN_, int DEPTH_, bool GATED_, bool DIRECT_> struct MmShape {
 	typedef E_ E;
 	static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_, DEPTH = DIRECT_ ? DEPTH_ : 2, THREADS = 64 * WM * WN;
@@ -295,17 +294,18 @@ __device__ __forceinline__ void mm_tile(const MmArgs& A, const Epi& epi, unsigne
 		if(DIRECT) {
 			char* const to = mm_smem + (t & (DEPTH - 1)) * BUF;
 			const bool out = k + piece >= K;
-			const unsigned vr = out ? MM_OUT : (unsigned) (lr * ldR + piece), vc = out ? MM_OUT : (unsigned) (lr * ldC + piece);
+			// (the step's place is part of the lane's offset: the descriptor's end is not held against the scalar one, and a last row's last 16 bytes may begin in front of it)
+			const unsigned vr = out ? MM_OUT : (unsigned) (lr * ldR + piece + k), vc = out ? MM_OUT : (unsigned) (lr * ldC + piece + k);
 #pragma unroll
 			for(int j = 0; j < (which & 1 ? LM : 0); j++) {
 				const int i = j * NW + wave;
-				__builtin_amdgcn_raw_ptr_buffer_load_lds(rRows, (__attribute__((address_space(3))) void*) (to + i * 1024), 16, (int) (vr + (unsigned) (i * 8 * ldR)), k, 0, 0);
+				__builtin_amdgcn_raw_ptr_buffer_load_lds(rRows, (__attribute__((address_space(3))) void*) (to + i * 1024), 16, (int) (vr + (unsigned) (i * 8 * ldR)), 0, 0, 0);
 			}
 #pragma unroll
 			for(int j = 0; j < (which & 2 ? LN : 0); j++) {
 				const int i = j * NW + wave;
 				__builtin_amdgcn_raw_ptr_buffer_load_lds(col_half(i) ? rUp : rCols, (__attribute__((address_space(3))) void*) (to + TM * 128 + i * 1024), 16,
-					(int) (vc + (unsigned) (col_row(i) * ldC)), k, 0, 0);
+					(int) (vc + (unsigned) (col_row(i) * ldC)), 0, 0, 0);
 			}
 		}
 		else {
