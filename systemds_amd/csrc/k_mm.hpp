@@ -294,18 +294,20 @@ __device__ __forceinline__ void mm_tile(const MmArgs& A, const Epi& epi, unsigne
 		if(DIRECT) {
 			char* const to = mm_smem + (t & (DEPTH - 1)) * BUF;
 			const bool out = k + piece >= K;
-			// (the step's place is part of the lane's offset: the descriptor's end is not held against the scalar one, and a last row's last 16 bytes may begin in front of it)
-			const unsigned vr = out ? MM_OUT : (unsigned) (lr * ldR + piece + k), vc = out ? MM_OUT : (unsigned) (lr * ldC + piece + k);
+			// (ENDS: the step's place is part of the lane's offset, since the descriptor's end is not held against the scalar one and a last row's last 16 bytes may begin in
+			// front of it; elsewhere it is the scalar one: 8-bit gated unit of 4096 x 4096 into 2 x 12288 390 and 385 us, gradients at 2 x 8192 in bf16 1489 and 1464)
+			const int kv = ENDS ? k : 0, ks = ENDS ? 0 : k;
+			const unsigned vr = out ? MM_OUT : (unsigned) (lr * ldR + piece + kv), vc = out ? MM_OUT : (unsigned) (lr * ldC + piece + kv);
 #pragma unroll
 			for(int j = 0; j < (which & 1 ? LM : 0); j++) {
 				const int i = j * NW + wave;
-				__builtin_amdgcn_raw_ptr_buffer_load_lds(rRows, (__attribute__((address_space(3))) void*) (to + i * 1024), 16, (int) (vr + (unsigned) (i * 8 * ldR)), 0, 0, 0);
+				__builtin_amdgcn_raw_ptr_buffer_load_lds(rRows, (__attribute__((address_space(3))) void*) (to + i * 1024), 16, (int) (vr + (unsigned) (i * 8 * ldR)), ks, 0, 0);
 			}
 #pragma unroll
 			for(int j = 0; j < (which & 2 ? LN : 0); j++) {
 				const int i = j * NW + wave;
 				__builtin_amdgcn_raw_ptr_buffer_load_lds(col_half(i) ? rUp : rCols, (__attribute__((address_space(3))) void*) (to + TM * 128 + i * 1024), 16,
-					(int) (vc + (unsigned) (col_row(i) * ldC)), 0, 0, 0);
+					(int) (vc + (unsigned) (col_row(i) * ldC)), ks, 0, 0);
 			}
 		}
 		else {
