@@ -99,39 +99,45 @@ template <class E>
 __device__ __forceinline__ int mm_col(int lane, int r) { return MmOp<E>::FR == 32 ? 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3) : mm_col16<E>(lane, r); }
 template <class E> struct MmGroup { static constexpr int value = std::is_same<E, double>::value ? 1 : 4; };
 
-// exp, 1 / x and tanh for values that are rounded to T: 16-bit results take the instructions for 2^x and 1 / x (a relative error below 2^-20 for arguments up to 16,
-// a thousandth of a bf16 rounding, a hundredth of an fp16 one), fp32 and fp64 the full functions.
+// exp and 1 / x for values that are rounded to T: 16-bit results take the instructions for 2^x and 1 / x (relative errors: 2^-22 of either, and 2^-23 |x| of the exponential, from its
+// argument's rounding), fp32 and fp64 the full functions.
 template <class T> struct MmMath {
 	typedef typename MmCalc<T>::type C;
-	static __device__ __forceinline__ C logistic(C x) { return C(1) / (C(1) + exp(-x)); } // (exp overflows to infinity, 1 / infinity is 0: the limit)
-	static __device__ __forceinline__ C gauss(C x) { return exp(C(-0.5) * x * x); }
-	static __device__ __forceinline__ C tanh_of(C x) { return tanh(x); }
+	static __device__ __forceinline__ C exp_of(C x) { return exp(x); }
+	static __device__ __forceinline__ C inverse(C x) { return C(1) / x; }
 };
 template <> struct MmMath<float> {
-	static __device__ __forceinline__ float logistic(float x) { return 1.0f / (1.0f + expf(-x)); }
-	static __device__ __forceinline__ float gauss(float x) { return expf(-0.5f * x * x); }
-	static __device__ __forceinline__ float tanh_of(float x) { return tanhf(x); }
+	static __device__ __forceinline__ float exp_of(float x) { return expf(x); }
+	static __device__ __forceinline__ float inverse(float x) { return 1.0f / x; }
 };
 struct MmMathShort {
-	static __device__ __forceinline__ float logistic(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * x)); }
-	static __device__ __forceinline__ float gauss(float x) { return __builtin_amdgcn_exp2f(-0.72134752044448170f * x * x); }
-	static __device__ __forceinline__ float tanh_of(float x) { return 2.0f * logistic(2.0f * x) - 1.0f; }
+	static __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(1.44269504088896341f * x); }
+	static __device__ __forceinline__ float inverse(float x) { return __builtin_amdgcn_rcpf(x); }
 };
 template <> struct MmMath<__bf16> : MmMathShort {};
 template <> struct MmMath<_Float16> : MmMathShort {};
-__device__ __forceinline__ float mm_erf(float x) { return erff(x); }
-__device__ __forceinline__ double mm_erf(double x) { return erf(x); }
+__device__ __forceinline__ float mm_erfc(float x) { return erfcf(x); }
+__device__ __forceinline__ double mm_erfc(double x) { return erfc(x); }
 
-// The activation of a gated unit (act: enum cla_act) and its derivative, for results of type T.
+// The logistic function, and of both signs of x: 1 - l(x) is l(-x), which a difference would lose where it is small. (exp overflows to infinity, 1 / infinity is 0: the limit.)
+template <class T, class C>
+__device__ __forceinline__ C mm_logistic(C x) { return MmMath<T>::inverse(C(1) + MmMath<T>::exp_of(-x)); }
+template <class T, class C>
+__device__ __forceinline__ void mm_logistics(C x, C& of, C& minus) {
+	const C e = MmMath<T>::exp_of(-fabs(x)), l = MmMath<T>::inverse(C(1) + e);
+	of = x < C(0) ? e * l : l; minus = x < C(0) ? l : e * l;
+}
+
+// The activation of a gated unit (act: enum cla_act) and its derivative, for results of type T. Each in a form that keeps its digits where it is small: Phi(x) = erfc(-x / sqrt 2) / 2,
+// (1 + tanh a) / 2 = l(2 a). (As 1 + erf, 1 + tanh and l (1 - l): gelu(-5) 4 %, its approximation there 30 %, the logistic function's derivative at 12 1 % off in fp32.)
 enum : int { ACT_SIGMOID = 0, ACT_SILU = 1, ACT_GELU = 2, ACT_GELU_TANH = 3, ACT_RELU = 4, ACT_NONE = 5 };
 template <class T, class C>
 __device__ __forceinline__ C mm_act(C x, int act) {
-	typedef MmMath<T> F;
 	switch(act) { // (uniform)
-		case ACT_SIGMOID: return F::logistic(x);
-		case ACT_SILU: return x * F::logistic(x);
-		case ACT_GELU: return C(0.5) * x * (C(1) + mm_erf(x * C(0.70710678118654752440)));
-		case ACT_GELU_TANH: return C(0.5) * x * (C(1) + F::tanh_of(C(0.79788456080286535588) * (x + C(0.044715) * x * x * x)));
+		case ACT_SIGMOID: return mm_logistic<T>(x);
+		case ACT_SILU: return x * mm_logistic<T>(x);
+		case ACT_GELU: return C(0.5) * x * mm_erfc(x * C(-0.70710678118654752440));
+		case ACT_GELU_TANH: return x * mm_logistic<T>(C(1.59576912160573071176) * (x + C(0.044715) * x * x * x));
 		case ACT_RELU: return x < C(0) ? C(0) : x; // (a NaN stays one)
 		default: return x;
 	}
@@ -139,19 +145,20 @@ __device__ __forceinline__ C mm_act(C x, int act) {
 // value and derivative
 template <class T, class C>
 __device__ __forceinline__ void mm_act_both(C x, int act, C& value, C& slope) {
-	typedef MmMath<T> F;
+	C l, m; // l(.), l(-.)
 	switch(act) {
-		case ACT_SIGMOID: { value = F::logistic(x); slope = value * (C(1) - value); break; }
-		case ACT_SILU: { const C s = F::logistic(x); value = x * s; slope = s * (C(1) + x * (C(1) - s)); break; }
+		case ACT_SIGMOID: { mm_logistics<T>(x, l, m); value = l; slope = l * m; break; }
+		case ACT_SILU: { mm_logistics<T>(x, l, m); value = x * l; slope = l * (C(1) + x * m); break; }
 		case ACT_GELU: {
-			const C p = C(0.5) * (C(1) + mm_erf(x * C(0.70710678118654752440)));
-			value = x * p; slope = p + x * F::gauss(x) * C(0.39894228040143267794);
+			const C p = C(0.5) * mm_erfc(x * C(-0.70710678118654752440));
+			value = x * p; slope = p + x * MmMath<T>::exp_of(C(-0.5) * x * x) * C(0.39894228040143267794);
 			break;
 		}
 		case ACT_GELU_TANH: {
-			const C c = C(0.79788456080286535588), t = F::tanh_of(c * (x + C(0.044715) * x * x * x));
-			value = C(0.5) * x * (C(1) + t);
-			slope = C(0.5) * (C(1) + t) + C(0.5) * x * (C(1) - t * t) * c * (C(1) + C(0.134145) * x * x);
+			mm_logistics<T>(C(1.59576912160573071176) * (x + C(0.044715) * x * x * x), l, m);
+			const C w = l * m; // (0 long before x * x leaves the range)
+			value = x * l;
+			slope = w > C(0) ? l + x * w * C(1.59576912160573071176) * (C(1) + C(0.134145) * x * x) : l;
 			break;
 		}
 		case ACT_RELU: { value = x < C(0) ? C(0) : x; slope = x > C(0) ? C(1) : C(0); break; }
