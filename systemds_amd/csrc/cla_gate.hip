@@ -35,6 +35,12 @@ GatePlan gate_plan(int type, int64_t m, int nIn, int nOut) {
 	p.joins = take(p.parts > 1 ? (int64_t) p.parts * 2 * F * nIn * calc : 0);
 	p.sums = take((int64_t) p.sumRows * 2 * F * calc);
 	p.sums64 = take((int64_t) p.sumJoins * 2 * F * calc);
+	if(type == CLA_F16) {
+		p.normY = take(m * 4);
+		p.normW = take(2 * F * 4);
+		p.mostRow = take(m * 4);
+		p.mostCol = take(2 * F * 4);
+	}
 	p.bytes = at;
 	return p;
 }

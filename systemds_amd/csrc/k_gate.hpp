@@ -24,7 +24,9 @@ struct GatePlan {
 	int64_t kPartY; int32_t partsY;     // dY: bytes of the columns of P summed at a time (a multiple of 128)
 	int64_t kPart; int32_t parts;       // dW: rows of the batch summed at a time (a multiple of 256)
 	int32_t sumRows, sumJoins;          // dB: partial sums of a wave's or block's rows (at most so many), and of 64 of those
-	size_t P, Pt, Wt, Yt, joinsY, joins, sums, sums64, bytes;
+	size_t P, Pt, Wt, Yt, joinsY, joins, sums, sums64;
+	size_t normY, normW, mostRow, mostCol; // fp16: norms of the rows of Y and W, bounds of the rows and columns of P
+	size_t bytes;
 };
 
 GatePlan gate_plan(int type, int64_t m, int nIn, int nOut);

@@ -6,7 +6,9 @@
 //   dY = [dG dU] [Wg; Wu],   dW = t([dG dU]) Y,   db = column sums of [dG dU]
 // together; then the sums that were split.
 // The tiles want both operands by rows of the summed index, so dG and dU are written by row and by column, W and Y are transposed into the workspace. dG and dU are
-// rounded to T between the products: the matrix cores take no wider operand, and a rounding of 2^-8 (bf16) of each of many terms leaves less than the result's own.
+// rounded to T between the products: the matrix cores take operands of 16 bits at 8 times the rate of fp32, and both operands of one type. Independent roundings of a sum's terms leave as much, relative to
+// the result, as one of the result does, so the gradients of Y and W are off by 1.4 times the latter alone (bf16, 2-norm: 0.0023 of 0.0017); as a sum of two 16-bit values each the two products would take
+// twice their time, two thirds of the call. fp16 has too few exponents for that: a row (for dY) or column (for dW) of them is brought into range by a power of two that the product takes back.
 // Sums over the batch for few weights are split into parts, joined in their order: results do not depend on timing.
 //
 // Bound, and what was measured. Few rows: the bytes of the weights, bf16 4 x 4096 into 2 x 12288 39 us (5.2 TB/s). Many: the tiles (k_mm.hpp), bf16 4096 x 4096 into 2 x 12288 651 - 674 us
@@ -78,14 +80,15 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_gate_few(GateFew<T> A) {
 			red[i] = dG; red[MR * 256 + i] = dU; // (of the first wave's sums nothing but this thread's are read at this place)
 			const int64_t half = B.ldP / 2, m = m0 + row, pad = 16 / (int) sizeof(T);
 			if(B.P && row < rows && col < half) {
-				B.P[m * B.ldP + col] = (T) dG;
-				B.P[m * B.ldP + half + col] = (T) dU;
+				const C by = B.row_power(m);
+				B.P[m * B.ldP + col] = (T) (dG * by);
+				B.P[m * B.ldP + half + col] = (T) (dU * by);
 			}
 			if(B.Pt && col < A.nOut && m < (A.m + pad - 1) / pad * pad) {
 				const int64_t part = m / B.kPart;
 				T* const to = B.Pt + part * 2 * A.nOut * B.kPart + (m - part * B.kPart);
-				to[col * B.kPart] = (T) dG;
-				to[(col + A.nOut) * B.kPart] = (T) dU;
+				to[col * B.kPart] = (T) (dG * B.col_power(col));
+				to[(col + A.nOut) * B.kPart] = (T) (dU * B.col_power(col + A.nOut));
 			}
 		}
 	}
@@ -344,10 +347,116 @@ template <> struct MmBits<float> { typedef uint32_t type; };
 template <> struct MmBits<__bf16> { typedef uint16_t type; };
 template <> struct MmBits<_Float16> { typedef uint16_t type; };
 
+// fp16: bounds of dG and dU, whose magnitudes may leave the type's range (above, or below where their sums do not) though the gradients do not:
+//   |dG| <= 1.13 |D| (|y| |wu| + |bu|),   |dU| <= |D| max(|y| |wg| + |bg|, 1)
+// of the 2-norms of the rows of Y and W (a derivative of an activation is at most 1.13, a value at most its argument or 1); up to sqrt(nIn) above what is there, which costs as much of the 2^39 between
+// the bound and the last place left. An output that D leaves out (0) bounds nothing.
+// Cost, both kernels and the products' rows: 4096 x 4096 into 2 x 8192 93 us of 1625, 4 x 1245 into 977 12 of 41.
+// TPR threads to a row.
+template <int TPR>
+__global__ __launch_bounds__(256) void k_gate_norms(const _Float16* __restrict__ Y, int64_t m, int64_t ldY, const _Float16* __restrict__ W, int64_t rowsW, int64_t ldW, int K,
+	float* __restrict__ normY, float* __restrict__ normW, uint32_t* __restrict__ mostRow, uint32_t* __restrict__ mostCol) {
+	constexpr int ROWS = 256 / TPR;
+	const int t = threadIdx.x % TPR;
+	for(int64_t row = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR; row < m + rowsW; row += (int64_t) gridDim.x * ROWS) {
+		const bool ofY = row < m;
+		const _Float16* const x = ofY ? Y + row * ldY : W + (row - m) * ldW;
+		float s = 0.0f;
+		for(int k = t * 8; k < K; k += TPR * 8) {
+			const mm_f16x8 p = __builtin_bit_cast(mm_f16x8, mm_load16<2>((const char*) (x + k), (int64_t) (K - k) * 2));
+#pragma unroll
+			for(int v = 0; v < 8; v++) s = fmaf((float) p[v], (float) p[v], s);
+		}
+#pragma unroll
+		for(int d = TPR / 2; d > 0; d >>= 1) s += __shfl_xor(s, d, TPR);
+		if(t == 0) {
+			if(ofY) { normY[row] = sqrtf(s); mostRow[row] = 0; }
+			else { normW[row - m] = sqrtf(s); mostCol[row - m] = 0; }
+		}
+	}
+}
+
+// A block takes 512 columns of `steps` times 64 rows, its waves 8 rows at a time: a block to a CU, since what costs is that they meet at the columns' maxima (4096 x 8192 38 us, a block for every
+// 64 rows 57). Rows and columns behind the last ones are the last ones again, which changes no maximum. (A largest magnitude does not depend on the order: the bits of what is not negative, those
+// of NaN above all others.) WIDE: rows of 8 values or more.
+template <bool WIDE>
+__global__ __launch_bounds__(512) void k_gate_bounds(const _Float16* __restrict__ D, int64_t ldD, int64_t m, int N, const _Float16* __restrict__ bias, const float* __restrict__ normY,
+	const float* __restrict__ normW, uint32_t* __restrict__ mostRow, uint32_t* __restrict__ mostCol, int64_t steps) {
+	__shared__ uint32_t part[8][16][65];
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, colRuns = (N + 511) / 512;
+	const int64_t step0 = (int64_t) (blockIdx.x / (unsigned) colRuns) * steps;
+	const int first = (int) (blockIdx.x % (unsigned) colRuns) * 512, c0 = WIDE ? min(first + lane * 8, N - 8) : 0;
+	float wg[8], wu[8], bg[8], bu[8];
+	uint32_t most[16]; // (gate's columns, the other projection's)
+#pragma unroll
+	for(int v = 0; v < 8; v++) {
+		const int c = min(c0 + v, N - 1);
+		wg[v] = normW[c]; wu[v] = 1.13f * normW[c + N];
+		bg[v] = bias ? fabsf((float) bias[c]) : 0.0f; bu[v] = bias ? 1.13f * fabsf((float) bias[c + N]) : 0.0f;
+		most[v] = most[8 + v] = 0;
+	}
+	for(int64_t step = step0; step < step0 + steps; step++) {
+		const int64_t r0 = step * 64 + wave * 8;
+		if(r0 >= m) break; // (uniform)
+		mm_f16x8 d[8];
+		float ny[8];
+		uint32_t row[8];
+#pragma unroll
+		for(int i = 0; i < 8; i++) {
+			const int64_t at = min(r0 + i, m - 1);
+			if(WIDE) __builtin_memcpy(&d[i], D + at * ldD + c0, 16);
+			else {
+#pragma unroll
+				for(int v = 0; v < 8; v++) d[i][v] = D[at * ldD + min(v, N - 1)];
+			}
+			ny[i] = normY[at];
+		}
+#pragma unroll
+		for(int i = 0; i < 8; i++) {
+			row[i] = 0;
+#pragma unroll
+			for(int v = 0; v < 8; v++) {
+				const float a = fabsf((float) d[i][v]);
+				const uint32_t p = __float_as_uint(a * fmaf(ny[i], wu[v], bu[v])), q = __float_as_uint(a * fmaxf(fmaf(ny[i], wg[v], bg[v]), 1.0f));
+				most[v] = max(most[v], p); most[8 + v] = max(most[8 + v], q);
+				row[i] = max(row[i], max(p, q));
+			}
+		}
+		// the lanes' largest of 8 rows: each half of the lanes keeps half of the rows, three times over; row[0] is that of row lane / 8 in the end
+#pragma unroll
+		for(int s = 32, n = 4; n > 0; s >>= 1, n >>= 1) {
+			const bool high = (lane & s) != 0;
+#pragma unroll
+			for(int i = 0; i < n; i++) {
+				const uint32_t other = (uint32_t) __shfl_xor((int) (high ? row[i] : row[i + n]), s, 64);
+				row[i] = max(high ? row[i + n] : row[i], other);
+			}
+		}
+#pragma unroll
+		for(int s = 4; s > 0; s >>= 1) row[0] = max(row[0], (uint32_t) __shfl_xor((int) row[0], s, 64));
+		if((lane & 7) == 0 && r0 + (lane >> 3) < m && row[0] != 0) atomicMax(mostRow + r0 + (lane >> 3), row[0]);
+	}
+#pragma unroll
+	for(int v = 0; v < 16; v++) part[wave][v][lane] = most[v];
+	__syncthreads();
+	const int c = first + (int) threadIdx.x; // neighbouring threads, neighbouring columns: an atomic access is a line for 16 of them
+	if(c < N) {
+		const int l = threadIdx.x >> 3, v = WIDE ? c - min(first + l * 8, N - 8) : c;
+#pragma unroll
+		for(int h = 0; h < 2; h++) {
+			uint32_t x = 0;
+#pragma unroll
+			for(int w = 0; w < 8; w++) x = max(x, part[w][h * 8 + v][l]);
+			if(x != 0) atomicMax(mostCol + h * N + c, x);
+		}
+	}
+}
+
 // Where a product goes: T, or (parts > 1) partial sums. One type for both, so that one kernel holds either product.
 template <class T> struct GateOut {
-	MmEpiOut<T, false> whole;
-	MmEpiOut<typename MmCalc<T>::type, false> part;
+	static constexpr bool POWERS = MmEpiBack<T>::POWERS;
+	MmEpiOut<T, false, POWERS> whole;
+	MmEpiOut<typename MmCalc<T>::type, false, POWERS> part;
 	int32_t parts;
 	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
 	template <class E, int MF, int NF, bool GATED, class Acc>
@@ -355,9 +464,9 @@ template <class T> struct GateOut {
 		if(parts == 1) whole.template run<E, MF, NF, GATED>(acc, region, m0, n0, M, N, p, rowPart, lane);
 		else part.template run<E, MF, NF, GATED>(acc, region, m0, n0, M, N, p, rowPart, lane);
 	}
-	static GateOut of(T* out, int64_t ld, typename MmCalc<T>::type* joins, int64_t M, int64_t N, int parts) {
-		return {{nullptr, nullptr, nullptr, out, ld, ACT_NONE, 0},
-			{nullptr, nullptr, nullptr, joins, N, ACT_NONE, M * N}, parts};
+	static GateOut of(T* out, int64_t ld, typename MmCalc<T>::type* joins, int64_t M, int64_t N, int parts, const uint32_t* most) {
+		return {{(const float*) most, nullptr, nullptr, out, ld, ACT_NONE, 0},
+			{(const float*) most, nullptr, nullptr, joins, N, ACT_NONE, M * N}, parts};
 	}
 };
 
@@ -381,11 +490,27 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 	T* const Yt = (T*) (c.ws + p.Yt);
 	C* const sums = (C*) (c.ws + p.sums);
 	C* const sums64 = (C*) (c.ws + p.sums64);
+	uint32_t* const mostRow = (uint32_t*) (c.ws + p.mostRow);
+	uint32_t* const mostCol = (uint32_t*) (c.ws + p.mostCol);
 	const int64_t pad = (c.m + V - 1) / V * V;
 
 	// projections, dG and dU; W and Y the other way round
 	const MmArgs project = gate_args<T>(c);
-	const MmEpiBack<T> back{(const T*) c.bias, (const T*) c.D, c.ldD, c.dY ? P : nullptr, 2 * p.half, c.dW ? Pt : nullptr, p.kPart, c.dB ? sums : nullptr, c.act};
+	const MmEpiBack<T> back{(const T*) c.bias, (const T*) c.D, c.ldD, c.dY ? P : nullptr, 2 * p.half, c.dW ? Pt : nullptr, p.kPart, c.dB ? sums : nullptr, c.act, mostRow, mostCol};
+	if constexpr(MmEpiBack<T>::POWERS) {
+		if(c.dY || c.dW) {
+			float* const normY = (float*) (c.ws + p.normY);
+			float* const normW = (float*) (c.ws + p.normW);
+			auto norms = c.nIn <= 128 ? k_gate_norms<16> : k_gate_norms<64>;
+			const int64_t perBlock = c.nIn <= 128 ? 16 : 4;
+			norms<<<(unsigned) std::min<int64_t>((c.m + 2 * F + perBlock - 1) / perBlock, g_numCU * 8), 256, 0, stream>>>((const T*) c.Y, c.m, c.ldY, (const T*) c.W, 2 * F, c.ldW, c.nIn, normY, normW,
+				mostRow, mostCol);
+			auto bounds = F >= 8 ? k_gate_bounds<true> : k_gate_bounds<false>;
+			const int64_t colRuns = (F + 511) / 512, rowSteps = (c.m + 63) / 64, steps = (rowSteps * colRuns + g_numCU - 1) / g_numCU;
+			bounds<<<(unsigned) ((rowSteps + steps - 1) / steps * colRuns), 512, 0, stream>>>((const T*) c.D, c.ldD, c.m, c.nOut, (const T*) c.bias, normY, normW, mostRow, mostCol, steps);
+			CLA_HIP(hipGetLastError());
+		}
+	}
 	GateLayouts<U> lay{};
 	const int64_t one = (int64_t) 1 << 40; // (a single part)
 	if(c.dY)
@@ -416,7 +541,7 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 	B.M = c.dW ? 2 * F : 0; B.N = c.nIn; B.parts = p.parts;
 	C* const joinsY = (C*) (c.ws + p.joinsY);
 	C* const joinsW = (C*) (c.ws + p.joins);
-	const GateOut<T> outY = GateOut<T>::of((T*) c.dY, c.ldDY, joinsY, c.m, c.nIn, p.partsY), outW = GateOut<T>::of((T*) c.dW, c.ldDW, joinsW, 2 * F, c.nIn, p.parts);
+	const GateOut<T> outY = GateOut<T>::of((T*) c.dY, c.ldDY, joinsY, c.m, c.nIn, p.partsY, mostRow), outW = GateOut<T>::of((T*) c.dW, c.ldDW, joinsW, 2 * F, c.nIn, p.parts, mostCol);
 	const int waveRows = few ? 16 * gate_few_rows<T>(c.m, c.nOut) : gate_shape<T>(project, true) / 1000 / 2, sumRows = (int) ((c.m + waveRows - 1) / waveRows); // (of a row of partial sums: a block's or a wave's)
 	GateSums<C> first{sums, sums64, sumRows, (int32_t) (2 * F), (sumRows + 63) / 64, (unsigned) ((2 * F + 63) / 64)};
 	MmArgs both = A; // (the shape that suits both: as many tiles as they have together)

@@ -44,10 +44,17 @@ __device__ __forceinline__ void mm_store(T* to, const MmPack<T, V>& x, int cols)
 	}
 }
 
-// The sums, times a scale for each row and column (SCALED: sums of 8-bit products), plus a bias for each column; gated: activation of the
+// A power of two that brings magnitudes up to `most` (a float's bits) below 2^15, and what takes it back: within 2^-113 .. 2^120, so that both are ordinary numbers. 1 for
+// a bound that is not finite (what it bounds is not either).
+__device__ __forceinline__ float mm_pow2(uint32_t most, bool back) {
+	const int e = (int) (most >> 23), k = e >= 255 ? 0 : min(141 - e, 120);
+	return __uint_as_float((uint32_t) (127 + (back ? -k : k)) << 23);
+}
+
+// The sums, times a scale for each row and column (SCALED: sums of 8-bit products) or what takes back the power of two of each row (POWERS), plus a bias for each column; gated: activation of the
 // gate's times the other projection's. Rounded to T once.
-template <class T, bool SCALED> struct MmEpiOut {
-	const float* sRow;
+template <class T, bool SCALED, bool POWERS = false> struct MmEpiOut {
+	const float* sRow;  // (POWERS: the rows' bounds)
 	const float* sCol;
 	const T* bias;      // null: none
 	T* out;
@@ -76,7 +83,10 @@ template <class T, bool SCALED> struct MmEpiOut {
 				bi[h][v] = bias ? (C) bias[col] : C(0);
 			}
 #pragma unroll
-		for(int i = 0; i < (MF * FR + 63) / 64; i++) sr[i] = SCALED ? sRow[min(m0 + i * 64 + lane, M - 1)] : 1.0f;
+		for(int i = 0; i < (MF * FR + 63) / 64; i++) {
+			sr[i] = SCALED || POWERS ? sRow[min(m0 + i * 64 + lane, M - 1)] : 1.0f;
+			if(POWERS) sr[i] = mm_pow2(__float_as_uint(sr[i]), true);
+		}
 #pragma unroll
 		for(int j = 0; j < MF; j++) {
 			Reg::template put<MF>(region, acc, j, lane);
@@ -84,7 +94,7 @@ template <class T, bool SCALED> struct MmEpiOut {
 #pragma unroll 1
 			for(int r0 = 0; r0 < FR; r0 += 64 / PER) {
 				const int r = r0 + lane / PER;
-				const C s = SCALED ? (C) __shfl(sr[j * FR / 64], (j * FR + r) & 63, 64) : C(1);
+				const C s = SCALED || POWERS ? (C) __shfl(sr[j * FR / 64], (j * FR + r) & 63, 64) : C(1);
 				MmPack<T, V> x;
 #pragma unroll
 				for(int v = 0; v < V; v++) {
@@ -93,6 +103,7 @@ template <class T, bool SCALED> struct MmEpiOut {
 					for(int h = 0; h < H; h++) {
 						y[h] = (C) Reg::at(region, h, r, c)[v];
 						if(SCALED) y[h] *= s * sc[h][v];
+						if(POWERS) y[h] *= s;
 						y[h] += bi[h][v];
 					}
 					x.x[v] = (T) (GATED ? mm_act<T>(y[0], act) * y[H - 1] : y[0]);
@@ -106,7 +117,8 @@ template <class T, bool SCALED> struct MmEpiOut {
 
 // Backward pass of a gated unit: from the projections G, U (the sums) and the incoming gradient D to dG = D U act'(G) and dU = D act(G), rounded to T once.
 // They are written twice, by row (P: what dY sums over) and by column (Pt: what dW sums over, rows of the batch in parts of kPart), with zeros where
-// either is rounded up to whole 16 bytes; sums over the wave's rows, of the values before that rounding, for the biases' gradient.
+// either is rounded up to whole 16 bytes; sums over the wave's rows, of the values before that rounding, for the biases' gradient. fp16: a row of P and a column of Pt are multiplied by a power of
+// two before they are rounded (by their bounds, see k_gate_bounds), so that no magnitude leaves the type's range; the products take it back.
 template <class T> struct MmEpiBack {
 	typedef typename MmCalc<T>::type C;
 	const T* bias;      // null: none
@@ -118,6 +130,11 @@ template <class T> struct MmEpiBack {
 	int64_t kPart;      // a multiple of 256
 	C* sums;            // null: not wanted; [wave's rows][2 N]
 	int32_t act;
+	const uint32_t* mostRow; // fp16: bounds of the rows and of the 2 N columns (bits of floats)
+	const uint32_t* mostCol;
+	static constexpr bool POWERS = std::is_same<T, _Float16>::value;
+	__device__ __forceinline__ C row_power(int64_t m) const { return POWERS ? (C) mm_pow2(mostRow[m], false) : C(1); }
+	__device__ __forceinline__ C col_power(int c) const { return POWERS ? (C) mm_pow2(mostCol[c], false) : C(1); }
 
 	template <class E, int NF, bool GATED> static constexpr int region() { return MmRegion<E, NF, GATED>::BYTES; }
 	template <class E, int MF, int NF, bool GATED, class Acc>
@@ -145,6 +162,7 @@ template <class T> struct MmEpiBack {
 				const int r = r0 + lane / PER;
 				const bool in = row0 + r < M && c0 < cols;
 				const T* const d = D + (row0 + r) * ldD + n0 + c0;
+				const C by = POWERS && P ? row_power(min(row0 + r, M - 1)) : C(1);
 				MmPack<T, V> g, u, dv;
 				if(in && c0 + V <= cols) dv = mm_get<MmPack<T, V>>(d);
 				else {
@@ -159,7 +177,7 @@ template <class T> struct MmEpiBack {
 					const bool there = in && c0 + v < cols;
 					const C dG = there ? (C) dv.x[v] * y * slope : C(0), dU = there ? (C) dv.x[v] * value : C(0);
 					*Reg::at(region, 0, r, c0 + v) = dG; *Reg::at(region, 1, r, c0 + v) = dU;
-					g.x[v] = (T) dG; u.x[v] = (T) dU;
+					g.x[v] = (T) (dG * by); u.x[v] = (T) (dU * by);
 				}
 				if(P && row0 + r < M && c0 < half) {
 					T* const to = P + (row0 + r) * ldP + n0 + c0;
@@ -183,9 +201,10 @@ template <class T> struct MmEpiBack {
 				for(int i = lane; i < 2 * COLS * (FR / V); i += 64) {
 					const int r = (i % (FR / V)) * V, c = i / (FR / V) % COLS, h = i / (FR / V) / COLS;
 					if(c >= cols || row0 + r >= M) continue;
+					const C by = col_power(h * N + n0 + c);
 					MmPack<T, V> p;
 #pragma unroll
-					for(int v = 0; v < V; v++) p.x[v] = (T) *Reg::at(region, h, r + v, c);
+					for(int v = 0; v < V; v++) p.x[v] = (T) (*Reg::at(region, h, r + v, c) * by);
 					*(MmPack<T, V>*) (to + (int64_t) (h * N + n0 + c) * kPart + r) = p;
 				}
 			}
