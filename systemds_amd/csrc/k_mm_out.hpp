@@ -33,6 +33,18 @@ template <class E, int NF, bool GATED> struct MmRegion {
 	}
 };
 
+// A sum of 8-bit products times its row's and column's scales. In fp32 their product may leave the range though the result does not (a sum of 2^25 with scales of 2^-70 each; a sum of 0 with
+// scales of 2^100): in 64 bits then.
+template <class C>
+__device__ __forceinline__ C mm_scaled_wide(C sum, C s, C t) { return (C) ((double) sum * (double) s * (double) t); }
+template <class C>
+__device__ __forceinline__ bool mm_scales_fit(C least, C most) { return sizeof(C) == 8 || (least >= C(1.17549435e-38f) && most <= C(3.4028234663852886e38f)); } // (not of a NaN)
+template <class C>
+__device__ __forceinline__ C mm_scaled(C sum, C s, C t) {
+	const C p = s * t, a = fabs(p);
+	return mm_scales_fit(a, a) ? sum * p : mm_scaled_wide(sum, s, t);
+}
+
 // V values to a row of the output, `cols` of them there: 16 bytes at once wherever the row begins.
 template <class T, int V>
 __device__ __forceinline__ void mm_store(T* to, const MmPack<T, V>& x, int cols) {
@@ -72,7 +84,7 @@ template <class T, bool SCALED, bool POWERS = false> struct MmEpiOut {
 		static_assert(64 % PER == 0 && FR * PER % 64 == 0, "a lane keeps its columns");
 		// a lane's columns are the same ones in every row: their scales and biases stay in registers; the scales of the wave's rows are held one by a lane
 		const int c = (lane % PER) * V, cols = N - n0 - c;
-		C sc[H][V], bi[H][V];
+		C sc[H][V], bi[H][V], least = C(INFINITY), most = C(0); // (magnitudes of the scales that are not 0)
 		float sr[(MF * FR + 63) / 64];
 #pragma unroll
 		for(int h = 0; h < H; h++)
@@ -81,37 +93,61 @@ template <class T, bool SCALED, bool POWERS = false> struct MmEpiOut {
 				const int col = min(n0 + c + v, N - 1) + h * N;
 				sc[h][v] = SCALED ? (C) sCol[col] : C(1);
 				bi[h][v] = bias ? (C) bias[col] : C(0);
+				if(SCALED) {
+					const C a = fabs(sc[h][v]);
+					least = a > C(0) ? fmin(least, a) : least; most = fmax(most, a);
+				}
 			}
 #pragma unroll
 		for(int i = 0; i < (MF * FR + 63) / 64; i++) {
 			sr[i] = SCALED || POWERS ? sRow[min(m0 + i * 64 + lane, M - 1)] : 1.0f;
 			if(POWERS) sr[i] = mm_pow2(__float_as_uint(sr[i]), true);
 		}
+		auto rows = [&](auto wide) {
 #pragma unroll
-		for(int j = 0; j < MF; j++) {
-			Reg::template put<MF>(region, acc, j, lane);
-			const int64_t row0 = m0 + j * FR;
+			for(int j = 0; j < MF; j++) {
+				Reg::template put<MF>(region, acc, j, lane);
+				const int64_t row0 = m0 + j * FR;
 #pragma unroll 1
-			for(int r0 = 0; r0 < FR; r0 += 64 / PER) {
-				const int r = r0 + lane / PER;
-				const C s = SCALED || POWERS ? (C) __shfl(sr[j * FR / 64], (j * FR + r) & 63, 64) : C(1);
-				MmPack<T, V> x;
+				for(int r0 = 0; r0 < FR; r0 += 64 / PER) {
+					const int r = r0 + lane / PER;
+					const C s = SCALED || POWERS ? (C) __shfl(sr[j * FR / 64], (j * FR + r) & 63, 64) : C(1);
+					MmPack<T, V> x;
 #pragma unroll
-				for(int v = 0; v < V; v++) {
-					C y[H];
+					for(int v = 0; v < V; v++) {
+						C y[H];
 #pragma unroll
-					for(int h = 0; h < H; h++) {
-						y[h] = (C) Reg::at(region, h, r, c)[v];
-						if(SCALED) y[h] *= s * sc[h][v];
-						if(POWERS) y[h] *= s;
-						y[h] += bi[h][v];
+						for(int h = 0; h < H; h++) {
+							y[h] = (C) Reg::at(region, h, r, c)[v];
+							if(SCALED) y[h] = decltype(wide)::value ? mm_scaled_wide(y[h], s, sc[h][v]) : y[h] * (s * sc[h][v]);
+							if(POWERS) y[h] *= s;
+							y[h] += bi[h][v];
+						}
+						x.x[v] = (T) (GATED ? mm_act<T>(y[0], act) * y[H - 1] : y[0]);
 					}
-					x.x[v] = (T) (GATED ? mm_act<T>(y[0], act) * y[H - 1] : y[0]);
+					if(row0 + r < M && cols > 0) mm_store<T, V>(out + part * zOut + (row0 + r) * ld + n0 + c, x, cols);
 				}
-				if(row0 + r < M && cols > 0) mm_store<T, V>(out + part * zOut + (row0 + r) * ld + n0 + c, x, cols);
+				mm_wave_sync();
 			}
-			mm_wave_sync();
+		};
+		if constexpr(SCALED && sizeof(C) == 4) { // (one way for the wave's whole tile: a choice for each row costs 5 % of the 8-bit gated unit)
+			C leastS = C(INFINITY), mostS = C(0);
+#pragma unroll
+			for(int i = 0; i < (MF * FR + 63) / 64; i++) {
+				const C a = fabs(sr[i]);
+				leastS = a > C(0) ? fmin(leastS, a) : leastS; mostS = fmax(mostS, a);
+			}
+#pragma unroll
+			for(int d = 32; d > 0; d >>= 1) {
+				leastS = fmin(leastS, __shfl_xor(leastS, d, 64)); mostS = fmax(mostS, __shfl_xor(mostS, d, 64));
+				least = fmin(least, __shfl_xor(least, d, 64)); most = fmax(most, __shfl_xor(most, d, 64));
+			}
+			if(__builtin_amdgcn_readfirstlane((int) !mm_scales_fit(leastS * least, mostS * most))) {
+				rows(std::true_type());
+				return;
+			}
 		}
+		rows(std::false_type());
 	}
 };
 

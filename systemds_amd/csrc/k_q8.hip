@@ -332,7 +332,7 @@ __global__ __launch_bounds__(64 * MMF_WAVES) void k_q8_few(Q8Few<T> A) {
 			int sum = 0;
 #pragma unroll
 			for(int w = 0; w < MMF_WAVES; w++) sum += red[(w * H + h) * MR * 256 + i];
-			x[h] = (C) sum * ((C) s * (C) A.t[col + h * A.N]);
+			x[h] = mm_scaled<C>((C) sum, (C) s, (C) A.t[col + h * A.N]);
 			if(A.bias) x[h] += (C) A.bias[col + h * A.N];
 		}
 		A.out[row * A.ld + col] = (T) (GATED ? mm_act<T>(x[0], A.act) * x[H - 1] : x[0]);
