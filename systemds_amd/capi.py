@@ -432,6 +432,26 @@ def build_block(n_rows, n_cols, specs):
     return b.finalize()
 
 
+def _matrix(a, rows, cols, what, dtype=np.float64):
+    """rows x cols values (rows None: any number of them) in C order, from an array of that shape or a flat one of whole rows: the library reads and writes so many."""
+    a = _arr(a, dtype)
+    if a.ndim == 1 and cols > 0 and a.size % cols == 0:
+        a = a.reshape(-1, cols)
+    if a.ndim != 2 or a.shape[1] != cols or (rows is not None and a.shape[0] != rows):
+        raise ClaError(ERR_INVALID, f"{what}: an array of {a.shape}, {'rows' if rows is None else rows} x {cols} wanted")
+    return a
+
+
+def _bias(bias, n):
+    return None if bias is None else _matrix(np.ravel(bias), 1, n, "bias").reshape(n)
+
+
+def _activation(act):
+    if isinstance(act, str) and act not in ACTIVATIONS:
+        raise ClaError(ERR_INVALID, f"unknown activation {act}")
+    return ACTIVATIONS[act] if isinstance(act, str) else int(act)
+
+
 # ---- products of layers: 8-bit matrices and gated units (pointers to device memory; types from TYPES, activations from ACTIVATIONS) ----
 def quantize_rows_dev_async(dY_ptr, type_, n_row_y, k, ldY, dQ_ptr, ldQ, dScale_ptr, stream=None):
     """cla_quantize_rows_dev_async: rows to 8 bits, a scale each."""
@@ -466,7 +486,7 @@ class ClaQ8:
 
     def set(self, W):
         """cla_q8_set: from fp64, n_rows x n_cols, quantised column by column."""
-        _check(self.lib.cla_q8_set(self.h, _ptr(_arr(W, np.float64).reshape(self.n_rows, self.n_cols))))
+        _check(self.lib.cla_q8_set(self.h, _ptr(_matrix(W, self.n_rows, self.n_cols, "W"))))
         return self
 
     def set_dev(self, dW_ptr, type_, ld, by_column=False):
@@ -475,7 +495,10 @@ class ClaQ8:
 
     def set_values(self, values, scales):
         """cla_q8_set_values: int8 values, n_rows x n_cols, and fp32 scales as they are."""
-        v, s = _arr(values, np.int8).reshape(self.n_rows, self.n_cols), _arr(scales, np.float32).reshape(self.n_cols)
+        v = _matrix(values, self.n_rows, self.n_cols, "values", np.int8)
+        if getattr(values, "dtype", None) != np.int8 and not np.array_equal(v, np.reshape(values, v.shape)):
+            raise ClaError(ERR_INVALID, "values: not all of them are 8-bit whole numbers")
+        s = _matrix(np.ravel(scales), 1, self.n_cols, "scales", np.float32)
         _check(self.lib.cla_q8_set_values(self.h, _ptr(v), _ptr(s)))
         return self
 
@@ -509,17 +532,15 @@ class ClaQ8:
 
     def lmm(self, Y, bias=None):
         """cla_q8_lmm: Y %*% W (+ bias) on host arrays; (out, number of non-zeros)."""
-        Y = _arr(Y, np.float64).reshape(-1, self.n_rows)
-        b = None if bias is None else _arr(bias, np.float64).reshape(self.n_cols)
+        Y, b = _matrix(Y, None, self.n_rows, "Y"), _bias(bias, self.n_cols)
         out = np.empty((Y.shape[0], self.n_cols), np.float64)
         return out, _check(self.lib.cla_q8_lmm(self.h, _ptr(Y), Y.shape[0], _ptr(b), _ptr(out)))
 
     def gate(self, act, Y, bias=None):
         """cla_q8_gate: act(Y %*% Wg) * (Y %*% Wu) on host arrays; (out, number of non-zeros)."""
-        Y = _arr(Y, np.float64).reshape(-1, self.n_rows)
-        b = None if bias is None else _arr(bias, np.float64).reshape(self.n_cols)
+        Y, b = _matrix(Y, None, self.n_rows, "Y"), _bias(bias, self.n_cols)
         out = np.empty((Y.shape[0], self.n_cols // 2), np.float64)
-        return out, _check(self.lib.cla_q8_gate(self.h, ACTIVATIONS[act] if isinstance(act, str) else act, _ptr(Y), Y.shape[0], _ptr(b), _ptr(out)))
+        return out, _check(self.lib.cla_q8_gate(self.h, _activation(act), _ptr(Y), Y.shape[0], _ptr(b), _ptr(out)))
 
 
 def gate_workspace(type_, n_row_y, n_in, n_out, backward):
@@ -540,26 +561,30 @@ def gate_backward_dev_async(act, type_, dY_ptr, n_row_y, n_in, ldY, dW_ptr, ldW,
                                                              ldGradY, dGradW_ptr, ldGradW, dGradBias_ptr, dWs_ptr, ws_bytes, stream))
 
 
+def _gate_operands(Y, W, bias):
+    W = _arr(W, np.float64)
+    if W.ndim != 2 or W.shape[0] % 2 or 0 in W.shape:
+        raise ClaError(ERR_INVALID, f"W: an array of {W.shape}, 2 n_out x n_in wanted")
+    return _matrix(Y, None, W.shape[1], "Y"), W, _bias(bias, W.shape[0])
+
+
 def gate(act, Y, W, bias=None):
     """cla_gate on host arrays, W 2 n_out x n_in: (out, number of non-zeros)."""
+    act, (Y, W, b) = _activation(act), _gate_operands(Y, W, bias)
     if not _initialised:
         init(0)
-    W = _arr(W, np.float64)
     n_in, n_out = W.shape[1], W.shape[0] // 2
-    Y = _arr(Y, np.float64).reshape(-1, n_in)
-    b = None if bias is None else _arr(bias, np.float64).reshape(2 * n_out)
     out = np.empty((Y.shape[0], n_out), np.float64)
-    return out, _check(load_library().cla_gate(ACTIVATIONS[act], _ptr(Y), Y.shape[0], n_in, _ptr(W), _ptr(b), n_out, _ptr(out)))
+    return out, _check(load_library().cla_gate(act, _ptr(Y), Y.shape[0], n_in, _ptr(W), _ptr(b), n_out, _ptr(out)))
 
 
 def gate_backward(act, Y, W, grad, bias=None):
     """cla_gate_backward on host arrays: (gradient of Y, of W, of bias)."""
+    act, (Y, W, b) = _activation(act), _gate_operands(Y, W, bias)
+    n_in, n_out = W.shape[1], W.shape[0] // 2
+    grad = _matrix(grad, Y.shape[0], n_out, "grad")
     if not _initialised:
         init(0)
-    W = _arr(W, np.float64)
-    n_in, n_out = W.shape[1], W.shape[0] // 2
-    Y, grad = _arr(Y, np.float64).reshape(-1, n_in), _arr(grad, np.float64).reshape(-1, n_out)
-    b = None if bias is None else _arr(bias, np.float64).reshape(2 * n_out)
     gy, gw, gb = np.empty_like(Y), np.empty_like(W), np.empty(2 * n_out)
-    _check(load_library().cla_gate_backward(ACTIVATIONS[act], _ptr(Y), Y.shape[0], n_in, _ptr(W), _ptr(b), n_out, _ptr(grad), _ptr(gy), _ptr(gw), _ptr(gb)))
+    _check(load_library().cla_gate_backward(act, _ptr(Y), Y.shape[0], n_in, _ptr(W), _ptr(b), n_out, _ptr(grad), _ptr(gy), _ptr(gw), _ptr(gb)))
     return gy, gw, gb
