@@ -314,6 +314,8 @@ class ClaBlock:
     def mmchain(self, v, w=None, ctype=0):
         v = _arr(v, np.float64).reshape(-1)
         w = None if w is None else _arr(w, np.float64).reshape(-1)
+        if v.size != self.n_cols or (ctype != 0 and w is not None and w.size != self.n_rows):
+            raise ClaError(ERR_INVALID, f"mmchain: vectors of {v.size} and {0 if w is None else w.size} values, {self.n_cols} and {self.n_rows} wanted")
         out = np.empty((self.n_cols,), np.float64)
         nnz = _check(self.lib.cla_mmchain(self.h, _ptr(v), _ptr(w), int(ctype), _ptr(out)))
         return out, nnz

@@ -83,3 +83,18 @@ def test_8_bit_matrix(rec):
     assert h.lmm(np.ones(14), np.ones(10))[0].shape == (2, 10) and h.gate(1, np.ones((3, 7)))[0].shape == (3, 5)
     assert [n for n, _ in rec.calls] == ["cla_q8_set", "cla_q8_set", "cla_q8_set_values", "cla_q8_lmm", "cla_q8_gate"]
     h.h = None
+
+
+def test_chain_of_a_block(rec):
+    """The multiply chain's vectors are as long as the block's columns and rows."""
+    from systemds_amd import capi
+    blk = object.__new__(capi.ClaBlock)
+    blk.lib, blk.h, blk.n_rows, blk.n_cols = rec, None, 9, 4
+    refused("mmchain", blk.mmchain, np.ones(3))
+    refused("mmchain", blk.mmchain, np.ones(5), np.ones(9), 1)
+    for ctype in (1, 2):
+        refused("mmchain", blk.mmchain, np.ones(4), np.ones(8), ctype)
+    assert rec.calls == []
+    blk.mmchain(np.ones((4, 1)))
+    blk.mmchain(np.ones(4), np.ones((9, 1)), 1)
+    assert [n for n, _ in rec.calls] == ["cla_mmchain", "cla_mmchain"]
