@@ -305,8 +305,9 @@ int cla_preagg(cla_handle h, int32_t group, const double* Y, int32_t nRowY, doub
  * What a network over the same data adds to the products above. Weights W are nRows x nCols as in Y %*% X: a row of Y has nRows values,
  * the output nCols. Operands and outputs are row-major with a leading dimension in elements, of one of the types below; device pointers are
  * aligned to their elements (8-bit rows of a product and workspaces to 16 bytes). Work is queued on a stream, nothing is allocated and nothing waited
- * for in the `_dev_async` forms (but for a block's first cla_block_quantize_rows_dev_async), so that they can be captured into a graph; workspaces belong to the caller: calls that may run at the same
- * time (other streams, other graphs) take workspaces of their own. Operands, outputs and workspaces do not overlap. nRowY may be 0. */
+ * for in the `_dev_async` forms (but for the chunks of cla_block_quantize_rows_dev_async), so that they can be captured into a graph; workspaces belong
+ * to the caller: calls that may run at the same time (other streams, other graphs) take workspaces of their own. Operands, outputs and workspaces do not
+ * overlap. nRowY may be 0. */
 enum cla_type { CLA_F64 = 0, CLA_F32 = 1, CLA_BF16 = 2, CLA_F16 = 3 };
 /* Activations: 1 / (1 + exp(-x)), x / (1 + exp(-x)), x Phi(x), its tanh approximation, max(x, 0), x. */
 enum cla_act { CLA_ACT_SIGMOID = 0, CLA_ACT_SILU = 1, CLA_ACT_GELU = 2, CLA_ACT_GELU_TANH = 3, CLA_ACT_RELU = 4, CLA_ACT_NONE = 5 };
@@ -317,8 +318,9 @@ enum cla_act { CLA_ACT_SIGMOID = 0, CLA_ACT_SILU = 1, CLA_ACT_GELU = 2, CLA_ACT_
 int cla_quantize_rows_dev_async(const void* dY, int32_t type, int64_t nRowY, int32_t k, int64_t ldY, int8_t* dQ, int64_t ldQ, float* dScale,
 	void* hipStream);
 /* The same for all rows of a compressed block, decoded in chunks on its stream: what a layer with many outputs takes instead of X %*% B. The first call
- * allocates the chunk (at most 64 MiB, kept until the block is freed), so it is not the one to capture. Returns 0 or a negative error without waiting
- * for the stream. */
+ * allocates the chunk (at most 64 MiB, kept until the block is freed); on the device a call begins behind the block's last one, whatever stream that was
+ * on. A call that is captured gets a chunk of its own, as large and kept as long, so that its graph may be replayed beside other graphs and calls of the
+ * block. Returns 0 or a negative error without waiting for the stream. */
 int cla_block_quantize_rows_dev_async(cla_handle h, int8_t* dQ, int64_t ldQ, float* dScale);
 
 /* An 8-bit matrix resident in HBM: W[k, j] = values[k, j] * scales[j]. nRows <= 131,071 (sums of products stay exact in 32 bits), nCols <= 2^21.

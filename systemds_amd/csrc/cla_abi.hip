@@ -346,6 +346,7 @@ void cla_block_free(cla_handle b) {
 	if(b->dStageOut) (void) hipFree(b->dStageOut);
 	if(b->dScratch) (void) hipFree(b->dScratch);
 	if(b->dQuantRows) (void) hipFree(b->dQuantRows);
+	if(b->quantDone) (void) hipEventDestroy(b->quantDone);
 	if(b->dChain) (void) hipFree(b->dChain);
 	if(b->dSdcPlan) (void) hipFree(b->dSdcPlan);
 	if(b->dSdcDesc) (void) hipFree(b->dSdcDesc);

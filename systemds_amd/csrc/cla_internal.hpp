@@ -191,10 +191,11 @@ struct cla_block {
 	double* dStageIn = nullptr; size_t stageInCap = 0;
 	double* dStageOut = nullptr; size_t stageOutCap = 0;
 	void* dScratch = nullptr;   size_t scratchCap = 0;
-	double* dQuantRows = nullptr;    // a chunk of decoded rows on their way to 8 bits: its size follows from the block's, so captured calls may keep it
+	double* dQuantRows = nullptr;    // a chunk of decoded rows on their way to 8 bits, and the end of its last use (on whatever stream that was); captured calls have chunks of their own (wsOld)
+	hipEvent_t quantDone = nullptr;
 	double* dLmmWs = nullptr;   size_t lmmWsCap = 0; bool lmmWsClean = false; // launch_lmm_joint: zeros between calls (k_take_block clears what a call has used)
 	double* dChain = nullptr;   size_t chainCap = 0;   // the multiply chain's own: X %*% v, or the sums of the blocks of its one kernel
-	std::vector<double*> wsOld;         // smaller ones of either of earlier calls
+	std::vector<double*> wsOld;         // smaller ones of either of earlier calls, and what captured calls hold
 	// exact code counts of all dictionary-coded groups (totalVals int32, group g at tblOff[g]),
 	// computed on the first TSMM and kept, like the reference's cached counts
 	// (CG/AColGroupValue.java getCounts)

@@ -200,14 +200,34 @@ int cla_block_quantize_rows_dev_async(cla_handle b, int8_t* dQ, int64_t ldQ, flo
 	std::lock_guard<std::recursive_mutex> lk(b->mu);
 	clear_stats(b);
 	const int64_t bytes = (int64_t) b->nCols * 8, chunk = std::min<int64_t>(b->nRows, std::max<int64_t>(1, ((int64_t) 64 << 20) / bytes));
-	if(!b->dQuantRows && (rc = device_room(what, (void**) &b->dQuantRows, (size_t) (chunk * bytes)))) return rc;
-	for(int64_t r0 = 0; r0 < b->nRows; r0 += chunk) {
-		const int64_t r1 = std::min(b->nRows, r0 + chunk);
-		if((rc = launch_decompress_rows(b, r0, r1, b->dQuantRows))) return rc;
-		Prof pf(b, "k_q8_rows", (long) (r1 - r0), 256, 0, (double) (r1 - r0) * (bytes + b->nCols + 4));
-		if((rc = launch_q8_rows(b->dQuantRows, CLA_F64, r1 - r0, b->nCols, b->nCols, dQ + r0 * ldQ, ldQ, dScale + r0, b->stream))) return rc;
+	// One chunk for the block's calls, each of which waits for the last use of it on the device (the block may have changed streams); one of its own for a call that is being
+	// captured, since its graph may be replayed beside any other.
+	hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+	CLA_HIP(hipStreamIsCapturing(b->stream, &capturing));
+	double* rows = b->dQuantRows;
+	if(capturing != hipStreamCaptureStatusNone) {
+		b->wsOld.reserve(b->wsOld.size() + 1);
+		hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed; // (an allocation is none of the stream's work)
+		CLA_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+		rc = device_room(what, (void**) &rows, (size_t) (chunk * bytes));
+		CLA_HIP(hipThreadExchangeStreamCaptureMode(&mode));
+		if(rc) return rc;
+		b->wsOld.push_back(rows);
 	}
-	return 0;
+	else {
+		if(!rows && (rc = device_room(what, (void**) &rows, (size_t) (chunk * bytes)))) return rc;
+		b->dQuantRows = rows;
+		if(b->quantDone) CLA_HIP(hipStreamWaitEvent(b->stream, b->quantDone, 0));
+		else CLA_HIP(hipEventCreateWithFlags(&b->quantDone, hipEventDisableTiming));
+	}
+	for(int64_t r0 = 0; r0 < b->nRows && !rc; r0 += chunk) {
+		const int64_t r1 = std::min(b->nRows, r0 + chunk);
+		if((rc = launch_decompress_rows(b, r0, r1, rows))) break;
+		Prof pf(b, "k_q8_rows", (long) (r1 - r0), 256, 0, (double) (r1 - r0) * (bytes + b->nCols + 4));
+		rc = launch_q8_rows(rows, CLA_F64, r1 - r0, b->nCols, b->nCols, dQ + r0 * ldQ, ldQ, dScale + r0, b->stream);
+	}
+	if(capturing == hipStreamCaptureStatusNone) CLA_HIP(hipEventRecord(b->quantDone, b->stream));
+	return rc;
 	CLA_CATCH_CODE(int)
 }
 
