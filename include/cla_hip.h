@@ -331,7 +331,7 @@ void cla_q8_free(cla_q8_handle h);
 int cla_q8_set_stream(cla_q8_handle h, void* hipStream);
 /* Sets the matrix from fp64 (host) or any type (device), each column quantised as cla_quantize_rows_dev_async does rows; or from values and scales
  * as they are (any int8). byColumn != 0: the array has a row per column (nCols x nRows, ld >= nRows), else it is nRows x nCols (ld >= nCols).
- * These wait for the handle's stream. */
+ * These wait for the handle's stream, and before they replace values for all work on the device, which may read the old ones. */
 int cla_q8_set(cla_q8_handle h, const double* W);
 int cla_q8_set_dev(cla_q8_handle h, const void* dW, int32_t type, int64_t ld, int32_t byColumn);
 int cla_q8_set_values(cla_q8_handle h, const int8_t* values, const float* scales);

@@ -80,6 +80,12 @@ static int check_q8(cla_q8* h, bool set) {
 	return check_ready();
 }
 
+// What is on its way on a stream that the handle was on before, or in a graph's replay, still reads the values that are about to be replaced.
+static int wait_for_readers(cla_q8* h) {
+	if(h->set) CLA_HIP(hipDeviceSynchronize());
+	return 0;
+}
+
 struct DevTmp { // device memory of a call that waits
 	void* p = nullptr;
 	~DevTmp() { if(p) (void) hipFree(p); }
@@ -288,6 +294,7 @@ int cla_q8_set_dev(cla_q8_handle h, const void* dW, int32_t type, int64_t ld, in
 	if((rc = check_operand(what, "W", dW, byColumn ? h->nCols : h->nRows, byColumn ? h->nRows : h->nCols, ld, es, es))) return rc;
 	std::lock_guard<std::recursive_mutex> lk(h->mu);
 	DevTmp tmp;
+	if((rc = wait_for_readers(h))) return rc;
 	if(byColumn) rc = launch_q8_rows(dW, type, h->nCols, (int) h->nRows, ld, h->dW, h->ldW, h->dScale, h->stream);
 	else {
 		if((rc = device_room(what, &tmp.p, (size_t) h->nRows * h->nCols * 8))) return rc;
@@ -326,7 +333,7 @@ int cla_q8_set_values_dev(cla_q8_handle h, const int8_t* dValues, int64_t ld, in
 		(rc = check_operand(what, "the scales", dScales, 1, h->nCols, h->nCols, 4, 4)))
 		return rc;
 	std::lock_guard<std::recursive_mutex> lk(h->mu);
-	if((rc = launch_q8_layout(dValues, ld, byColumn, h->nRows, h->nCols, h->dW, h->ldW, h->stream))) return rc;
+	if((rc = wait_for_readers(h)) || (rc = launch_q8_layout(dValues, ld, byColumn, h->nRows, h->nCols, h->dW, h->ldW, h->stream))) return rc;
 	CLA_HIP(hipMemcpyAsync(h->dScale, dScales, sizeof(float) * (size_t) h->nCols, hipMemcpyDeviceToDevice, h->stream));
 	CLA_HIP(hipStreamSynchronize(h->stream));
 	h->set = true;

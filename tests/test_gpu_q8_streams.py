@@ -127,3 +127,36 @@ def test_chunks_go_with_the_block(cla):
         once()
     assert free_device_bytes() > before - (64 << 20)
     ok(lib.hipStreamDestroy(s))
+
+
+def test_values_replaced_while_products_are_on_their_way(cla):
+    """Products queued on one stream see the values that the matrix had, though it is on another stream when they are replaced; later ones the new values."""
+    rng = np.random.default_rng(4)
+    lib, (a, b), m, k, n = hip(), streams(2), 4096, 4096, 4096
+    Y = DevBuf.from_numpy(rng.standard_normal((m, k)).astype(np.float32))
+    h = cla.ClaQ8(k, n)
+    W = [rng.integers(-127, 128, (k, n)).astype(np.int8) for _ in range(2)]
+    scales = np.ones(n, np.float32)
+    ws, want = DevBuf(h.workspace(m)), []
+    for w in W:
+        h.set_values(w, scales)
+        o = DevBuf(m * n * 4)
+        h.lmm_dev_async(Y.ptr, 1, m, k, None, o.ptr, n, ws.ptr, ws.nbytes)
+        ok(lib.hipDeviceSynchronize())
+        want.append(o.to_numpy((m, n), np.float32))
+    dW, dS = [DevBuf.from_numpy(np.ascontiguousarray(w.T)) for w in W], DevBuf.from_numpy(scales)
+    outs = [DevBuf(m * n * 4) for _ in range(6)]
+    for turn in range(2):
+        h.set_values_dev(dW[0].ptr, k, dS.ptr, True)
+        h.set_stream(a.value)
+        for o in outs[:5]:
+            h.lmm_dev_async(Y.ptr, 1, m, k, None, o.ptr, n, ws.ptr, ws.nbytes)
+        h.set_stream(b.value)
+        h.set_values_dev(dW[1].ptr, k, dS.ptr, True)
+        h.lmm_dev_async(Y.ptr, 1, m, k, None, outs[5].ptr, n, ws.ptr, ws.nbytes)
+        ok(lib.hipDeviceSynchronize())
+        for i, o in enumerate(outs):
+            assert np.array_equal(o.to_numpy((m, n), np.float32), want[i == 5])
+    h.close()
+    for s in (a, b):
+        ok(lib.hipStreamDestroy(s))
