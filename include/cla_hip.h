@@ -362,7 +362,7 @@ int64_t cla_q8_gate(cla_q8_handle h, int32_t act, const double* Y, int64_t nRowY
 
 /* The gated unit in the operands' own type: out[nRowY x nOut] = act(Y %*% t(Wg) + bg) * (Y %*% t(Wu) + bu), W = rbind(Wg, Wu): 2 nOut x nIn, a row of
  * weights per output column; bias (2 nOut) may be null. 16-bit and fp32 operands are summed in fp32, fp64 in fp64. One kernel. At most 4 MiB a row
- * of Y and 1 MiB a row of the output, rows of Y and W at most 2 GiB apart. The workspace holds cla_gate_workspace(type, nRowY, nIn, nOut, 0) bytes (0: it may be null). */
+ * of Y and 1 MiB a row of the output, rows of Y and W at most 2 GiB apart; gradients of fewer than 2^30 rows. The workspace holds cla_gate_workspace(type, nRowY, nIn, nOut, 0) bytes (0: it may be null). */
 int64_t cla_gate_workspace(int32_t type, int64_t nRowY, int32_t nIn, int32_t nOut, int32_t backward);
 int cla_gate_dev_async(int32_t act, int32_t type, const void* dY, int64_t nRowY, int32_t nIn, int64_t ldY, const void* dW, int64_t ldW,
 	const void* dBias, int32_t nOut, void* dOut, int64_t ldOut, void* dWorkspace, int64_t workspaceBytes, void* hipStream);

@@ -45,14 +45,25 @@ GatePlan gate_plan(int type, int64_t m, int nIn, int nOut) {
 	return p;
 }
 
-int launch_gate(const GateCall& c, hipStream_t stream) {
-	if(c.m == 0) return 0;
+static int launch_rows(const GateCall& c, hipStream_t stream) {
 	switch(c.type) {
 		case CLA_F64: return gate_forward<double>(c, stream);
 		case CLA_F32: return gate_forward<float>(c, stream);
 		case CLA_BF16: return gate_forward<__bf16>(c, stream);
 		default: return gate_forward<_Float16>(c, stream);
 	}
+}
+
+int launch_gate(const GateCall& c, hipStream_t stream) {
+	const int64_t es = (int64_t) type_bytes(c.type), rows = rows_of_a_launch(64, 64, 2 * (int64_t) c.nOut); // (tiles of the smallest shape)
+	for(int64_t r = 0; r < c.m; r += rows) {
+		GateCall part = c;
+		part.m = std::min(c.m - r, rows);
+		part.Y = (const char*) c.Y + r * c.ldY * es;
+		part.out = (char*) c.out + r * c.ldOut * es;
+		if(const int rc = launch_rows(part, stream)) return rc;
+	}
+	return 0;
 }
 
 int launch_gate_backward(const GateCall& c, hipStream_t stream) {

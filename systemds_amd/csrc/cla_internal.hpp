@@ -279,6 +279,7 @@ struct cla_block {
 namespace cla {
 
 void set_error(const char* fmt, ...);
+constexpr int64_t LAUNCH_THREADS = 0xffffffffLL; // threads of a launch along x that the runtime takes (blocks times threads)
 int check_ready(); // cla_init has been called, and the device it chose is the current one
 extern int g_ldsPerBlock;   // usable LDS bytes per workgroup
 // Lets a kernel take up to the device's LDS per workgroup as dynamic shared memory; said once per kernel (a value

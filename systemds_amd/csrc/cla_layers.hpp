@@ -13,6 +13,8 @@ int check_rows(const char* what, int64_t m);
 int check_operand(const char* what, const char* name, const void* p, int64_t rows, int64_t cols, int64_t ld, size_t es, size_t to);
 // Device memory for a call; where there is none, the runtime's error does not stay for the next call to find.
 int device_room(const char* what, void** p, size_t bytes);
+// Rows that one launch of tiles of tm x tn on 256 threads takes of a product with so many columns (shapes with more threads have as much larger tiles).
+inline int64_t rows_of_a_launch(int64_t tm, int64_t tn, int64_t cols) { return LAUNCH_THREADS / 256 / ((cols + tn - 1) / tn) * tm; }
 // Non-zeros of n values on the device; waits for the stream.
 int64_t count_nonzero(const double* x, int64_t n, unsigned long long* dCount, hipStream_t stream);
 

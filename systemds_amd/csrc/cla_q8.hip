@@ -91,7 +91,7 @@ struct DevTmp { // device memory of a call that waits
 	~DevTmp() { if(p) (void) hipFree(p); }
 };
 
-static int product(cla_q8* h, const char* what, bool gated, int act, const int8_t* Q, int64_t ldQ, const float* s, int64_t m, const void* bias, void* out, int type,
+static int product(cla_q8* h, bool gated, int act, const int8_t* Q, int64_t ldQ, const float* s, int64_t m, const void* bias, void* out, int type,
 	int64_t ldOut, const void* Y = nullptr, int64_t ldY = 0) {
 	Q8Product p{};
 	p.W = h->dW; p.ldW = h->ldW; p.t = h->dScale;
@@ -99,9 +99,14 @@ static int product(cla_q8* h, const char* what, bool gated, int act, const int8_
 	p.K = (int32_t) h->nRows; p.N = h->nCols; p.act = act;
 	p.bias = bias; p.out = out; p.ldOut = ldOut;
 	p.Y = Y; p.ldY = ldY;
-	const int64_t n = h->nCols; // (tiles of the smallest shape)
-	if(((m + 63) / 64) * ((n + 63) / 64) > 0x7fffffffLL) { set_error("%s: %lld x %lld outputs", what, (long long) m, (long long) n); return -CLA_ERR_UNSUPPORTED; }
-	return launch_q8(p, type, gated, h->stream);
+	const int64_t rows = rows_of_a_launch(64, 128, h->nCols); // (tiles of the smallest shape)
+	for(int64_t r = 0; r < m; r += rows) {
+		p.m = std::min(m - r, rows);
+		if(Q) { p.Q = Q + r * ldQ; p.s = s + r; }
+		p.out = (char*) out + r * ldOut * (int64_t) type_bytes(type);
+		if(const int rc = launch_q8(p, type, gated, h->stream)) return rc;
+	}
+	return 0;
 }
 
 static int check_out(cla_q8* h, const char* what, bool gated, int act, int64_t m, const void* bias, const void* out, int type, int64_t ldOut) {
@@ -127,12 +132,12 @@ static int from_rows(cla_q8* h, const char* what, bool gated, int act, const voi
 		return -CLA_ERR_INVALID;
 	}
 	std::lock_guard<std::recursive_mutex> lk(h->mu);
-	if(q8_fuses(m, h->nRows)) return product(h, what, gated, act, nullptr, 0, nullptr, m, dBias, dOut, type, ldOut, dY, ldY);
+	if(q8_fuses(m, h->nRows)) return product(h, gated, act, nullptr, 0, nullptr, m, dBias, dOut, type, ldOut, dY, ldY);
 	float* const s = (float*) ws;
 	int8_t* const q = (int8_t*) ws + up((size_t) m * sizeof(float), 256);
 	const int64_t ldQ = ld_rows(h);
 	if((rc = launch_q8_rows(dY, type, m, (int) h->nRows, ldY, q, ldQ, s, h->stream))) return rc;
-	return product(h, what, gated, act, q, ldQ, s, m, dBias, dOut, type, ldOut);
+	return product(h, gated, act, q, ldQ, s, m, dBias, dOut, type, ldOut);
 }
 
 static int from_quantized(cla_q8* h, const char* what, bool gated, int act, const int8_t* dQ, int64_t ldQ, const float* dScale, int64_t m, const void* dBias, void* dOut,
@@ -143,7 +148,7 @@ static int from_quantized(cla_q8* h, const char* what, bool gated, int act, cons
 	if((rc = check_operand(what, "the 8-bit rows", dQ, m, h->nRows, ldQ, 1, 16)) || (rc = check_operand(what, "the rows' scales", dScale, m, 1, 1, 4, 4))) return rc;
 	if(ldQ & 15 || ldQ > ((int64_t) 4 << 20)) { set_error("%s: 8-bit rows are a multiple of 16 bytes apart, at most 4 MiB (%lld)", what, (long long) ldQ); return -CLA_ERR_INVALID; }
 	std::lock_guard<std::recursive_mutex> lk(h->mu);
-	return product(h, what, gated, act, dQ, ldQ, dScale, m, dBias, dOut, type, ldOut);
+	return product(h, gated, act, dQ, ldQ, dScale, m, dBias, dOut, type, ldOut);
 }
 
 // The host forms: operands and result staged on the device, the workspace behind them.

@@ -157,9 +157,9 @@ static int64_t gate_tiles(MmArgs& A) {
 	return (int64_t) A.tilesM * A.tilesN * A.parts;
 }
 
-static inline int gate_grid(int64_t blocks) {
-	if(blocks <= 0x7fffffffLL) return 0;
-	set_error("gate: a product of %lld tiles", (long long) blocks);
+static inline int gate_grid(int64_t blocks, int threads) {
+	if(blocks <= LAUNCH_THREADS / threads) return 0;
+	set_error("gate: a launch of %lld blocks of %d threads (fewer rows at a time)", (long long) blocks, threads);
 	return -CLA_ERR_UNSUPPORTED;
 }
 
@@ -186,7 +186,7 @@ static int gate_project(MmArgs A, const Epi& epi, int64_t moreBlocks, const More
 	auto launch = [&](auto s) {
 		typedef decltype(s) Shape;
 		const int64_t blocks = gate_tiles<Shape>(A);
-		if(const int rc = gate_grid(blocks + moreBlocks)) return rc;
+		if(const int rc = gate_grid(blocks + moreBlocks, Shape::THREADS)) return rc;
 		auto kernel = k_mm_and<Shape, Epi, More>;
 		CLA_HIP(allow_full_lds((const void*) kernel));
 		kernel<<<(unsigned) (blocks + moreBlocks), Shape::THREADS, std::max(Shape::template lds<Epi>(), More::LDS), stream>>>(A, epi, (unsigned) blocks, more);
@@ -225,7 +225,7 @@ struct GateTranspose {
 	unsigned blocksR, blocks;   // 0 blocks: nothing to do
 	static GateTranspose of(const void* src, int64_t ld, int64_t R, int cols, void* dst, int64_t ldDst, int64_t zDst, int64_t padR, int64_t kPart) {
 		const int64_t r = (padR + 63) / 64;
-		return {src, ld, R, cols, dst, ldDst, zDst, padR, kPart, (unsigned) r, (unsigned) (r * ((cols + 63) / 64))};
+		return {src, ld, R, cols, dst, ldDst, zDst, padR, kPart, (unsigned) r, (unsigned) std::min<int64_t>(r * ((cols + 63) / 64), 0x7fffffffLL)};
 	}
 };
 
@@ -497,6 +497,14 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 	// projections, dG and dU; W and Y the other way round
 	const MmArgs project = gate_args<T>(c);
 	const MmEpiBack<T> back{(const T*) c.bias, (const T*) c.D, c.ldD, c.dY ? P : nullptr, 2 * p.half, c.dW ? Pt : nullptr, p.kPart, c.dB ? sums : nullptr, c.act, mostRow, mostCol};
+	GateLayouts<U> lay{};
+	const int64_t one = (int64_t) 1 << 40; // (a single part)
+	if(c.dY)
+		for(int h = 0; h < 2; h++)
+			lay.t[h] = GateTranspose::of((const T*) c.W + h * F * c.ldW, c.ldW, F, c.nIn, Wt + h * p.half, 2 * p.half, 0, p.half, one);
+	if(c.dW) lay.t[2] = GateTranspose::of(c.Y, c.ldY, c.m, c.nIn, Yt, p.kPart, c.nIn * p.kPart, pad, p.kPart);
+	int64_t lays = (int64_t) lay.t[0].blocks + lay.t[1].blocks + lay.t[2].blocks;
+	if((rc = gate_grid(lays, 256))) return rc;
 	if constexpr(MmEpiBack<T>::POWERS) {
 		if(c.dY || c.dW) {
 			float* const normY = (float*) (c.ws + p.normY);
@@ -511,20 +519,12 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 			CLA_HIP(hipGetLastError());
 		}
 	}
-	GateLayouts<U> lay{};
-	const int64_t one = (int64_t) 1 << 40; // (a single part)
-	if(c.dY)
-		for(int h = 0; h < 2; h++)
-			lay.t[h] = GateTranspose::of((const T*) c.W + h * F * c.ldW, c.ldW, F, c.nIn, Wt + h * p.half, 2 * p.half, 0, p.half, one);
-	if(c.dW) lay.t[2] = GateTranspose::of(c.Y, c.ldY, c.m, c.nIn, Yt, p.kPart, c.nIn * p.kPart, pad, p.kPart);
 	// few of them behind the projections' tiles, in the same launch; many in one of their own: a tile's LDS leaves a CU to one block (4096 x 4096 into 2 x 8192 on
 	// bf16 1.85 ms in all, 1.50 so)
-	int64_t lays = (int64_t) lay.t[0].blocks + lay.t[1].blocks + lay.t[2].blocks;
 	// (so few results that tiles would take a handful of CUs; more are written by column faster from a tile, and the layouts ride along: 59 x 4055 into 174 in fp64 277 us on
 	// tiles, 72 so, 76 x 256 into 2560 44 and 53)
 	const bool few = (c.m + 15) / 16 * ((F + 15) / 16) <= g_numCU;
 	if(lays > (few ? 0 : 2 * g_numCU)) {
-		if((rc = gate_grid(lays))) return rc;
 		k_gate_layouts<U><<<(unsigned) lays, 256, 0, stream>>>(lay);
 		lays = 0;
 	}
@@ -551,7 +551,7 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 		constexpr int waves = Shape::THREADS / 64;
 		const int64_t nA = gate_tiles<Shape>(A), nB = gate_tiles<Shape>(B), nC = c.dB ? (int64_t) first.blocksC * ((first.groups + waves - 1) / waves) : 0;
 		if(nA + nB + nC == 0) return 0;
-		if(const int r = gate_grid(nA + nB + nC)) return r;
+		if(const int r = gate_grid(nA + nB + nC, Shape::THREADS)) return r;
 		auto kernel = k_mm_two<Shape, GateOut<T>, GateOut<T>, GateSums<C>>;
 		CLA_HIP(allow_full_lds((const void*) kernel));
 		kernel<<<(unsigned) (nA + nB + nC), Shape::THREADS, Shape::template lds<GateOut<T>>(), stream>>>(A, outY, (unsigned) nA, B, outW, (unsigned) nB, first);

@@ -145,15 +145,17 @@ static int q8_rows(const void* Yp, int64_t m, int K, int64_t ld, int8_t* Q, int6
 	// Short rows 16 threads each, 16 rows a block; up to 2 pieces a lane a wave holds the row and no barrier is needed; longer ones take a block, few rows, too
 	// (idle waves would be all they leave).
 	const int64_t pieces = (K + V - 1) / V;
-#define Q8_ROWS(TPR, NV) k_q8_rows<T, TPR, NV><<<(unsigned) ((m + 256 / TPR - 1) / (256 / TPR)), 256, 0, stream>>>(Y, m, K, ld, Q, ldQ, scale)
-	if(pieces <= 16) Q8_ROWS(16, 1);
-	else if(pieces <= 64) Q8_ROWS(16, 4);
+#define Q8_ROWS(TPR, NV) \
+	for(int64_t r = 0, rows = LAUNCH_THREADS / 256 * (256 / TPR); r < m; r += rows) \
+		k_q8_rows<T, TPR, NV><<<(unsigned) ((std::min(m - r, rows) + 256 / TPR - 1) / (256 / TPR)), 256, 0, stream>>>(Y + r * ld, std::min(m - r, rows), K, ld, Q + r * ldQ, ldQ, scale + r)
+	if(pieces <= 16) { Q8_ROWS(16, 1); }
+	else if(pieces <= 64) { Q8_ROWS(16, 4); }
 	else if(m < 1024 || pieces > 64 * 2) {
-		if(pieces <= 256 * 2) Q8_ROWS(256, 2);
-		else if(pieces <= 256 * 4) Q8_ROWS(256, 4);
-		else Q8_ROWS(256, 8);
+		if(pieces <= 256 * 2) { Q8_ROWS(256, 2); }
+		else if(pieces <= 256 * 4) { Q8_ROWS(256, 4); }
+		else { Q8_ROWS(256, 8); }
 	}
-	else Q8_ROWS(64, 2);
+	else { Q8_ROWS(64, 2); }
 #undef Q8_ROWS
 	CLA_HIP(hipGetLastError());
 	return 0;
