@@ -348,8 +348,9 @@ template <> struct MmBits<__bf16> { typedef uint16_t type; };
 template <> struct MmBits<_Float16> { typedef uint16_t type; };
 
 // fp16: bounds of dG and dU, whose magnitudes may leave the type's range (above, or below where their sums do not) though the gradients do not:
-//   |dG| <= 1.13 |D| (|y| |wu| + |bu|),   |dU| <= |D| max(|y| |wg| + |bg|, 1)
-// of the 2-norms of the rows of Y and W (a derivative of an activation is at most 1.13, a value at most its argument or 1); up to sqrt(nIn) above what is there, which costs as much of the 2^39 between
+//   |dG| <= 1.13 |D| (|y| |wu| + |bu|),   |dU| <= |D| max(|y| |wg| + bg, 1)
+// of the 2-norms of the rows of Y and W (a derivative of an activation is at most 1.13, a value at most its argument or 1, the logistic function's 1; a gate shut by a bias of -infinity bounds nothing;
+// without an activation |bg|); up to sqrt(nIn) above what is there, which costs as much of the 2^39 between
 // the bound and the last place left. An output that D leaves out (0) bounds nothing.
 // Cost, both kernels and the products' rows: 4096 x 4096 into 2 x 8192 93 us of 1625, 4 x 1245 into 977 12 of 41.
 // TPR threads to a row.
@@ -381,7 +382,7 @@ __global__ __launch_bounds__(256) void k_gate_norms(const _Float16* __restrict__
 // of NaN above all others.) WIDE: rows of 8 values or more.
 template <bool WIDE>
 __global__ __launch_bounds__(512) void k_gate_bounds(const _Float16* __restrict__ D, int64_t ldD, int64_t m, int N, const _Float16* __restrict__ bias, const float* __restrict__ normY,
-	const float* __restrict__ normW, uint32_t* __restrict__ mostRow, uint32_t* __restrict__ mostCol, int64_t steps) {
+	const float* __restrict__ normW, uint32_t* __restrict__ mostRow, uint32_t* __restrict__ mostCol, int64_t steps, int act) {
 	__shared__ uint32_t part[8][16][65];
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, colRuns = (N + 511) / 512;
 	const int64_t step0 = (int64_t) (blockIdx.x / (unsigned) colRuns) * steps;
@@ -391,8 +392,8 @@ __global__ __launch_bounds__(512) void k_gate_bounds(const _Float16* __restrict_
 #pragma unroll
 	for(int v = 0; v < 8; v++) {
 		const int c = min(c0 + v, N - 1);
-		wg[v] = normW[c]; wu[v] = 1.13f * normW[c + N];
-		bg[v] = bias ? fabsf((float) bias[c]) : 0.0f; bu[v] = bias ? 1.13f * fabsf((float) bias[c + N]) : 0.0f;
+		wg[v] = act == ACT_SIGMOID ? 0.0f : normW[c]; wu[v] = 1.13f * normW[c + N];
+		bg[v] = !bias || act == ACT_SIGMOID ? 0.0f : act == ACT_NONE ? fabsf((float) bias[c]) : (float) bias[c]; bu[v] = bias ? 1.13f * fabsf((float) bias[c + N]) : 0.0f;
 		most[v] = most[8 + v] = 0;
 	}
 	for(int64_t step = step0; step < step0 + steps; step++) {
@@ -515,7 +516,7 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 				mostRow, mostCol);
 			auto bounds = F >= 8 ? k_gate_bounds<true> : k_gate_bounds<false>;
 			const int64_t colRuns = (F + 511) / 512, rowSteps = (c.m + 63) / 64, steps = (rowSteps * colRuns + g_numCU - 1) / g_numCU;
-			bounds<<<(unsigned) ((rowSteps + steps - 1) / steps * colRuns), 512, 0, stream>>>((const T*) c.D, c.ldD, c.m, c.nOut, (const T*) c.bias, normY, normW, mostRow, mostCol, steps);
+			bounds<<<(unsigned) ((rowSteps + steps - 1) / steps * colRuns), 512, 0, stream>>>((const T*) c.D, c.ldD, c.m, c.nOut, (const T*) c.bias, normY, normW, mostRow, mostCol, steps, c.act);
 			CLA_HIP(hipGetLastError());
 		}
 	}

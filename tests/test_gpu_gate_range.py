@@ -111,3 +111,34 @@ def test_gradients_beyond_the_type_are_infinite(cla):
     assert not np.isfinite(g[0][5]).all() and not np.isnan(g[0]).any()
     rest = np.arange(40) != 5
     assert np.array_equal(g[0][rest], want[0][rest])
+
+
+@pytest.mark.parametrize("m,k,n", SHAPES)
+@pytest.mark.parametrize("kind", ["relu", "sigmoid"])
+def test_gates_shut_by_their_bias(cla, kind, m, k, n):
+    """Gates whose bias is -infinity give nothing; the others' gradients, dG up to 2^19, are what they are without them: each side rounds every dG and dU by half a step or by half of the last
+    place 2^39 below its row's or column's bound, and the result by half a step."""
+    from devmem import DevBuf
+    u = unit(m, k, n, 2.0 ** -10, 2.0 ** -14 * k ** 0.5, 2.0 ** 14 if kind == "relu" else 2.0 ** -4, 2.0 ** 12 if m < 1000 else 2.0 ** 11, kind=kind, bias=True)
+    u.b = np.zeros(2 * n)
+    u.b[n:] = 40.0 if kind == "relu" else 120.0
+    shut = np.arange(n) % 3 == 1
+    u.D[:, shut] = 0.0
+    u.dD, u.dB = held(u.D, T, n), DevBuf.from_numpy(encode(u.b, T))
+    clean = [o.get() for o in u.backward((True, True, False))[:2]]
+    g, p, _, _ = u.projections()
+    v, _, s, _ = value_and_slope(g, kind)
+    P = np.abs(np.concatenate([u.D * p * s, u.D * v], 1))
+    assert P.max() > 2 * 65504
+    u.D[:, shut] = 30000.0
+    u.b[:n][shut] = -np.inf
+    u.dD, u.dB = held(u.D, T, n), DevBuf.from_numpy(encode(u.b, T))
+    got = [o.get() for o in u.backward((True, True, False))[:2]]
+    y, w = np.linalg.norm(u.Y, axis=1)[:, None], np.linalg.norm(u.W, axis=1)[None, :]
+    most = np.abs(u.D) * np.maximum(1.13 * (y * w[:, n:] + u.b[n:]), y * w[:, :n] + 1)
+    last = 2.0 ** -38 * most
+    rows, cols = P * 2.0 ** -11 + last.max(1)[:, None], P * 2.0 ** -11 + last.max(0).repeat(2).reshape(n, 2).T.reshape(-1)[None, :]
+    for x, c, off in ((got[0], clean[0], rows @ np.abs(u.W)), (got[1], clean[1], cols.T @ np.abs(u.Y))):
+        assert np.isfinite(c).all() and np.median(np.abs(c)) > 0
+        near(x, c, 2.1 * (off + 2.0 ** -11 * np.abs(c) + TINY[T]))
+    assert not got[1][:n][shut].any() and not got[1][n:][shut].any()
