@@ -11,8 +11,8 @@
 // twice their time, two thirds of the call. fp16 has too few exponents for that: a row (for dY) or column (for dW) of them is brought into range by a power of two that the product takes back.
 // Sums over the batch for few weights are split into parts, joined in their order: results do not depend on timing.
 //
-// Bound, and what was measured. Few rows: the bytes of the weights, bf16 4 x 4096 into 2 x 12288 39 us (5.2 TB/s). Many: the tiles (k_mm.hpp), bf16 4096 x 4096 into 2 x 12288 651 - 674 us
-// (1.25 PFLOP/s), gradients at 2 x 8192 1465 - 1513 us: layouts 65, projections 550, both products 960. fp64 400,009 x 100 into 2 x 64 245 - 250 us: 133 of matrix instructions, which the logistic
+// Bound, and what was measured. Few rows: the bytes of the weights, bf16 4 x 4096 into 2 x 12288 39 us (5.2 TB/s). Many: the tiles (k_mm.hpp), bf16 4096 x 4096 into 2 x 12288 660 - 683 us
+// (1.25 PFLOP/s), gradients at 2 x 8192 1477 - 1573 us: layouts 65, projections 550, both products 960. fp64 400,009 x 100 into 2 x 64 245 - 250 us: 133 of matrix instructions, which the logistic
 // function's vector instructions add to.
 #pragma once
 #include "../../include/cla_hip.h"

@@ -32,8 +32,8 @@ typedef _Float16 mm_f16x8 __attribute__((ext_vector_type(8)));
 template <class T> struct MmCalc { typedef float type; };
 template <> struct MmCalc<double> { typedef double type; };
 
-// An operand type on the matrix cores. FR: rows of a fragment (16 bytes of FR rows in 64 lanes: 64 / FR pieces of the summed index);
-// place(r): the fragment's column of a lane's result r, less what col(lane) adds.
+// An operand type on the matrix cores. FR: rows of a fragment (16 bytes of FR rows in 64 lanes: 64 / FR pieces of the summed index). A lane's results belong to row lane % FR of the rows' operand
+// and to the columns mm_col(lane, r) of the other, MmGroup of them next to each other.
 template <class E> struct MmOp;
 template <> struct MmOp<int8_t> {
 	static constexpr int FR = 32;
@@ -435,11 +435,10 @@ __device__ __forceinline__ void mm_tile(const MmArgs& A, const Epi& epi, unsigne
 }
 #endif
 
-// 1: a wave to a SIMD and all its registers; the others leave room for two
-template <class Shape> constexpr int mm_waves() { return Shape::THREADS == 256 && Shape::TM * Shape::TN >= 256 * 256 ? 1 : 2; }
+constexpr int MM_WAVES = 2; // waves to a SIMD that the registers leave room for
 
 template <class Shape, class Epi>
-__global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm(MmArgs A, Epi epi) {
+__global__ __launch_bounds__(Shape::THREADS, MM_WAVES) void k_mm(MmArgs A, Epi epi) {
 #ifdef __HIP_DEVICE_COMPILE__
 	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
 	mm_tile<Shape>(A, epi, blockIdx.x, gridDim.x, mm_smem);
@@ -448,7 +447,7 @@ __global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm(MmArgs
 
 // A product and other work in one launch: blocks below `blocks` take its tiles, `more` gets the others, counted from 0.
 template <class Shape, class Epi, class More>
-__global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm_and(MmArgs A, Epi epi, unsigned blocks, More more) {
+__global__ __launch_bounds__(Shape::THREADS, MM_WAVES) void k_mm_and(MmArgs A, Epi epi, unsigned blocks, More more) {
 #ifdef __HIP_DEVICE_COMPILE__
 	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
 	if(blockIdx.x < blocks) mm_tile<Shape>(A, epi, blockIdx.x, blocks, mm_smem);
@@ -458,7 +457,7 @@ __global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm_and(Mm
 
 // Two products and other work in one launch.
 template <class Shape, class EpiA, class EpiB, class More>
-__global__ __launch_bounds__(Shape::THREADS, mm_waves<Shape>()) void k_mm_two(MmArgs A, EpiA epiA, unsigned blocksA, MmArgs B, EpiB epiB, unsigned blocksB, More more) {
+__global__ __launch_bounds__(Shape::THREADS, MM_WAVES) void k_mm_two(MmArgs A, EpiA epiA, unsigned blocksA, MmArgs B, EpiB epiB, unsigned blocksB, More more) {
 #ifdef __HIP_DEVICE_COMPILE__
 	extern __shared__ __attribute__((aligned(16))) char mm_smem[];
 	const unsigned b = blockIdx.x;
@@ -480,7 +479,8 @@ template <class E>
 static inline bool mm_few_suits(int64_t m, int64_t n, int cus) {
 	return m <= 16 || (m + 15) / 16 * ((n + 15) / 16) <= (sizeof(E) == 1 ? 6 : sizeof(E) == 2 ? 4 : 8) * (int64_t) cus;
 }
-// How many rows (in sixteens) a block takes: up to 64, as few as it needs to give every CU one (48 where that holds all: 37 x 5001 into 7681 in 8 bits 17.5 us with 64, 16.9 so).
+// How many rows (in sixteens) a block takes: up to 64, as few as it needs to give every CU one (48 where that holds all: 37 rows, us
+// with 48 / without: bf16 gated 4096 into 2 x 4096 21 / 30, into 2 x 4864 37 / 40, fp32 62 / 83 and 107 / 111, 8-bit 5001 into 7681 22 / 26, 8-bit gated 4096 into 2 x 4096 16 / 21).
 static inline int mm_few_rows(int64_t m, int64_t n, int cus) {
 	for(int r = 4; r > 1; r--)
 		if(m > 16 * (r - 1) && (r != 3 || m <= 48) && (m + 16 * r - 1) / (16 * r) * ((n + 15) / 16) >= cus) return r;

@@ -3,9 +3,9 @@
 // and the gated unit act(out of the first half of the columns) * (out of the second half), one kernel. The sums of 8-bit products are exact in 32 bits
 // (at most 131,071 terms of 128 * 128), so an output carries the roundings of its scales' products and its own.
 //
-// Bound, and what was measured (bf16 rows unless said otherwise). Few rows: the bytes of the weights, 1 x 4096 into 2 x 12288 25 us (4 TB/s), 1 x 4096 into 4096 6.2 us (the launch and two
-// round trips to memory). Many: tiles of 256 x 256, 4096 x 4096 into 2 x 12288 gated 380 - 390 us with 13 of them for the rows' quantisation (2.1 POP/s; the matrix cores are
-// busy 55 % of the cycles at 1.85 GHz), 8192 x 8192 into 8192 510 us. A short sum and a wide result: the result's bytes, 100,003 x 100 into 512 fp64 84 us (4.9 TB/s) behind 31 us of quantisation.
+// Bound, and what was measured (bf16 rows unless said otherwise). Few rows: the bytes of the weights, 1 x 4096 into 2 x 12288 26 us (3.9 TB/s; 30 us with weights that no cache holds), 1 x 4096 into 4096 6.3 us (the launch and two
+// round trips to memory). Many: tiles of 256 x 256, 4096 x 4096 into 2 x 12288 gated 381 - 399 us with 13 of them for the rows' quantisation (2.1 POP/s; the matrix cores are
+// busy 55 % of the cycles at 1.85 GHz), 8192 x 8192 into 8192 511 - 530 us. A short sum and a wide result: the result's bytes, 100,003 x 100 into 512 fp64 84 us (4.9 TB/s) behind 31 us of quantisation.
 #include "../../include/cla_hip.h"
 #include "k_q8.hpp"
 #include "k_mm_out.hpp"
