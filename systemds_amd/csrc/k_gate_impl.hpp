@@ -269,10 +269,11 @@ template <class U> struct GateLayouts {
 	}
 };
 
-template <class U>
-__global__ __launch_bounds__(256) void k_gate_layouts(GateLayouts<U> lay) {
+template <class U, class More>
+__global__ __launch_bounds__(256) void k_gate_layouts(GateLayouts<U> lay, unsigned blocks, More more) {
 	__shared__ __attribute__((aligned(16))) char smem[GateLayouts<U>::LDS];
-	lay.run(blockIdx.x, smem);
+	if(blockIdx.x < blocks) lay.run(blockIdx.x, smem);
+	else more.run(blockIdx.x - blocks, smem);
 }
 
 // Sums of 64 rows of partial sums at a time: a block takes 64 columns of them, its waves 64 rows each.
@@ -352,30 +353,44 @@ template <> struct MmBits<_Float16> { typedef uint16_t type; };
 // of the 2-norms of the rows of Y and W (a derivative of an activation is at most 1.13, a value at most its argument or 1, the logistic function's 1; a gate shut by a bias of -infinity bounds nothing;
 // without an activation |bg|); up to sqrt(nIn) above what is there, which costs as much of the 2^39 between
 // the bound and the last place left. An output that D leaves out (0) bounds nothing.
-// Cost, both kernels and the products' rows: 4096 x 4096 into 2 x 8192 93 us of 1625, 4 x 1245 into 977 12 of 41.
-// TPR threads to a row.
-template <int TPR>
-__global__ __launch_bounds__(256) void k_gate_norms(const _Float16* __restrict__ Y, int64_t m, int64_t ldY, const _Float16* __restrict__ W, int64_t rowsW, int64_t ldW, int K,
-	float* __restrict__ normY, float* __restrict__ normW, uint32_t* __restrict__ mostRow, uint32_t* __restrict__ mostCol) {
-	constexpr int ROWS = 256 / TPR;
-	const int t = threadIdx.x % TPR;
-	for(int64_t row = (int64_t) blockIdx.x * ROWS + threadIdx.x / TPR; row < m + rowsW; row += (int64_t) gridDim.x * ROWS) {
-		const bool ofY = row < m;
-		const _Float16* const x = ofY ? Y + row * ldY : W + (row - m) * ldW;
-		float s = 0.0f;
-		for(int k = t * 8; k < K; k += TPR * 8) {
-			const mm_f16x8 p = __builtin_bit_cast(mm_f16x8, mm_load16<2>((const char*) (x + k), (int64_t) (K - k) * 2));
+// Cost, both kernels and the products' rows: 4096 x 4096 into 2 x 8192 63 us of 1605, 4 x 1245 into 977 9 of 38 (the norms behind the layouts; in a launch of their own 103 and 12).
+struct GateNorms {
+	const _Float16* Y; int64_t m, ldY;
+	const _Float16* W; int64_t rowsW, ldW;
+	int32_t K;
+	float* normY; float* normW;
+	uint32_t* mostRow; uint32_t* mostCol;   // cleared on the way
+	unsigned blocks;
+	template <int TPR> __device__ __forceinline__ void rows(unsigned block) const { // TPR threads to a row
+		constexpr int ROWS = 256 / TPR;
+		const int t = threadIdx.x % TPR;
+		for(int64_t row = (int64_t) block * ROWS + threadIdx.x / TPR; row < m + rowsW; row += (int64_t) blocks * ROWS) {
+			const bool ofY = row < m;
+			const _Float16* const x = ofY ? Y + row * ldY : W + (row - m) * ldW;
+			float s = 0.0f;
+			for(int k = t * 8; k < K; k += TPR * 8) {
+				const mm_f16x8 p = __builtin_bit_cast(mm_f16x8, mm_load16<2>((const char*) (x + k), (int64_t) (K - k) * 2));
 #pragma unroll
-			for(int v = 0; v < 8; v++) s = fmaf((float) p[v], (float) p[v], s);
-		}
+				for(int v = 0; v < 8; v++) s = fmaf((float) p[v], (float) p[v], s);
+			}
 #pragma unroll
-		for(int d = TPR / 2; d > 0; d >>= 1) s += __shfl_xor(s, d, TPR);
-		if(t == 0) {
-			if(ofY) { normY[row] = sqrtf(s); mostRow[row] = 0; }
-			else { normW[row - m] = sqrtf(s); mostCol[row - m] = 0; }
+			for(int d = TPR / 2; d > 0; d >>= 1) s += __shfl_xor(s, d, TPR);
+			if(t == 0) {
+				if(ofY) { normY[row] = sqrtf(s); mostRow[row] = 0; }
+				else { normW[row - m] = sqrtf(s); mostCol[row - m] = 0; }
+			}
 		}
 	}
-}
+	__device__ __forceinline__ void run(unsigned block, char*) const {
+		if(K <= 128) rows<16>(block);
+		else rows<64>(block);
+	}
+	static GateNorms of(const GateCall& c, float* normY, float* normW, uint32_t* mostRow, uint32_t* mostCol) {
+		const int64_t n = c.m + 2 * (int64_t) c.nOut, perBlock = c.nIn <= 128 ? 16 : 4;
+		return {(const _Float16*) c.Y, c.m, c.ldY, (const _Float16*) c.W, 2 * (int64_t) c.nOut, c.ldW, c.nIn, normY, normW, mostRow, mostCol,
+			(unsigned) std::min<int64_t>((n + perBlock - 1) / perBlock, g_numCU * 8)};
+	}
+};
 
 // A block takes 512 columns of `steps` times 64 rows, its waves 8 rows at a time: a block to a CU, since what costs is that they meet at the columns' maxima (4096 x 8192 38 us, a block for every
 // 64 rows 57). Rows and columns behind the last ones are the last ones again, which changes no maximum. (A largest magnitude does not depend on the order: the bits of what is not negative, those
@@ -505,15 +520,14 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 			lay.t[h] = GateTranspose::of((const T*) c.W + h * F * c.ldW, c.ldW, F, c.nIn, Wt + h * p.half, 2 * p.half, 0, p.half, one);
 	if(c.dW) lay.t[2] = GateTranspose::of(c.Y, c.ldY, c.m, c.nIn, Yt, p.kPart, c.nIn * p.kPart, pad, p.kPart);
 	int64_t lays = (int64_t) lay.t[0].blocks + lay.t[1].blocks + lay.t[2].blocks;
-	if((rc = gate_grid(lays, 256))) return rc;
-	if constexpr(MmEpiBack<T>::POWERS) {
+	if((rc = gate_grid(lays + g_numCU * 8, 256))) return rc; // (the norms' blocks are at most so many)
+	if constexpr(MmEpiBack<T>::POWERS) { // (the layouts ride along with the norms)
 		if(c.dY || c.dW) {
 			float* const normY = (float*) (c.ws + p.normY);
 			float* const normW = (float*) (c.ws + p.normW);
-			auto norms = c.nIn <= 128 ? k_gate_norms<16> : k_gate_norms<64>;
-			const int64_t perBlock = c.nIn <= 128 ? 16 : 4;
-			norms<<<(unsigned) std::min<int64_t>((c.m + 2 * F + perBlock - 1) / perBlock, g_numCU * 8), 256, 0, stream>>>((const T*) c.Y, c.m, c.ldY, (const T*) c.W, 2 * F, c.ldW, c.nIn, normY, normW,
-				mostRow, mostCol);
+			const GateNorms norms = GateNorms::of(c, normY, normW, mostRow, mostCol);
+			k_gate_layouts<U><<<(unsigned) lays + norms.blocks, 256, 0, stream>>>(lay, (unsigned) lays, norms);
+			lays = 0;
 			auto bounds = F >= 8 ? k_gate_bounds<true> : k_gate_bounds<false>;
 			const int64_t colRuns = (F + 511) / 512, rowSteps = (c.m + 63) / 64, steps = (rowSteps * colRuns + g_numCU - 1) / g_numCU;
 			bounds<<<(unsigned) ((rowSteps + steps - 1) / steps * colRuns), 512, 0, stream>>>((const T*) c.D, c.ldD, c.m, c.nOut, (const T*) c.bias, normY, normW, mostRow, mostCol, steps, c.act);
@@ -526,7 +540,7 @@ int gate_backward(const GateCall& c, hipStream_t stream) {
 	// tiles, 72 so, 76 x 256 into 2560 44 and 53)
 	const bool few = (c.m + 15) / 16 * ((F + 15) / 16) <= g_numCU;
 	if(lays > (few ? 0 : 2 * g_numCU)) {
-		k_gate_layouts<U><<<(unsigned) lays, 256, 0, stream>>>(lay);
+		k_gate_layouts<U><<<(unsigned) lays, 256, 0, stream>>>(lay, (unsigned) lays, GateNothing());
 		lays = 0;
 	}
 	if(few) rc = gate_few<T, true>(GateFew<T>{(const T*) c.Y, c.ldY, (const T*) c.W, c.ldW, c.m, c.nIn, c.nOut, c.act, (const T*) c.bias, nullptr, 0, back}, stream);
